@@ -68,12 +68,12 @@ def draw(rng):
         case |= {"G": rng.choice([1, 2, 5, 8, 13, 16, 32, 64]), "skew": rng.choice([0.0, 0.5, 1.0]),
                  "tail": rng.choice([0, 0, 1, 100])}
         case["K"], case["N"] = min(case["K"], 4096), min(case["N"], 4096)
-        case["T"] = max(case["T"], case["tail"])
+        case["T"] = max(case["T"], case["tail"] + 1)                  # at least one row belongs to a group
     if kind.endswith("train"):
         case["wdtype"] = rng.choice(["f32", "bf16"])
         case["T"] = max(case["T"], 128)
     while work(case)["flops"] > 1.0e12:                               # no more than linear_prefill
-        case["T"] = max(case["T"] // 2, case.get("tail", 0))
+        case["T"] = max(case["T"] // 2, case.get("tail", 0) + 1)
     return case
 
 
