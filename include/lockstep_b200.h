@@ -410,6 +410,75 @@ int ls_mxfp4_linear_noalloc(const void *x, int x_dtype, const uint8_t *w_pk, con
                             void *c, int out_dtype, int64_t M, int64_t N, int64_t K,
                             int32_t *status, void *stream);
 
+/* ---- FP8 with one scale per block of 128 ------------------------------------
+ * (extension; lockstep has no 8-bit product.)  Codes are E4M3; a block's scale
+ * is the smallest power of two s with amax <= 448 s over its finite values, at
+ * least 2^-126, and 1 for a block of zeros; infinities and NaNs become E4M3's
+ * NaN.  Blocks are 128 values along the axis a product sums over, 128 x 128 for
+ * weights; a ragged end is a short block.  Sizes are free: only the row pitch
+ * `ld` of the codes (bytes) must be a multiple of 16.
+ *
+ * Scale bytes (UE8M0) lie in the tensor-core layout of the MXFP4 products: 512
+ * bytes per 128 rows x 4 blocks.  ls_fp8_sf_bytes gives the size for a
+ * [rows, K] operand with blocks along K.
+ *
+ * Ragged groups: `offsets` is a device array of groups + 1 ints; group g holds
+ * rows offsets[g] .. offsets[g + 1].  Its rows are cut into tiles of 128 from
+ * its first row on, tile i in row slot offsets[g] / 128 + g + i; there are
+ * ls_fp8_slots(rows, groups) slots, and scale buffers (and the column-wise
+ * codes) of a grouped tensor have that many times 128 rows.  Offsets must not
+ * decrease; others give unspecified values, never an access out of bounds.
+ * groups <= 1024. */
+int64_t ls_fp8_sf_bytes(int64_t rows, int64_t K);
+int64_t ls_fp8_slots(int64_t rows, int64_t groups);
+
+/* x [rows, K] (LS_F32 / LS_BF16) -> codes [rows, K] with blocks along K; scale
+ * (fp32 [rows, ceil(K / 128)]) and sf (ls_fp8_sf_bytes(rows, K), with offsets
+ * ls_fp8_sf_bytes(128 * slots, K)) may be NULL.  With offsets the codes keep
+ * x's row order and rows of no group are not written. */
+int ls_quantize_fp8(const void *x, int dtype, int64_t rows, int64_t K, const int *offsets, int64_t groups,
+                    uint8_t *codes, int64_t ld, float *scale, uint8_t *sf, void *stream);
+
+/* The same (codes, sf; both may be NULL) and the column-wise form (codes_t,
+ * sf_t: blocks of 128 rows) from one read of x.  codes_t is [rows, K] in x's
+ * orientation, with offsets [128 * slots, K] in slot order with zeros behind a
+ * group's last row; sf_t is ls_fp8_sf_bytes(K, rows), with offsets
+ * ls_fp8_sf_bytes(K, 128 * slots).  ld is the pitch of both. */
+int ls_quantize_fp8_both(const void *x, int dtype, int64_t rows, int64_t K, const int *offsets, int64_t groups,
+                         uint8_t *codes, uint8_t *sf, uint8_t *codes_t, uint8_t *sf_t, int64_t ld, void *stream);
+
+/* w [matrices, N, K] -> codes with one scale per 128 x 128; scale fp32
+ * [matrices, ceil(N / 128), ceil(K / 128)], sf (matrices times
+ * ls_fp8_sf_bytes(N, K)) and sf_t (of the transposes: ls_fp8_sf_bytes(K, N)
+ * each) may be NULL.  matrices <= 1024. */
+int ls_quantize_fp8_weight(const void *w, int dtype, int64_t matrices, int64_t N, int64_t K, uint8_t *codes,
+                           int64_t ld, float *scale, uint8_t *sf, uint8_t *sf_t, void *stream);
+
+/* out[r, c] = codes[r, c] * scale[r / row_block, c / 128]; row_block = 1 or 128 */
+int ls_dequantize_fp8(const uint8_t *codes, int64_t ld, const float *scale, int64_t rows, int64_t K, int row_block,
+                      void *out, int out_dtype, void *stream);
+
+/* Products, C row-major contiguous [M, N] in out_dtype:
+ *   form 0  C = A[M, K] B[N, K]^T    sfa of A, sfb of B along K       (forward)
+ *   form 1  C = A[M, K] B[K, N]      sfb = B's sf_t                   (input gradient)
+ *   form 2  C = A[K, M]^T B[K, N]    column-wise operands and sf_t's  (weight gradient)
+ * lda, ldb: row pitches in bytes.  Every pointer is 16-byte aligned. */
+int ls_fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t ldb, const uint8_t *sfa,
+                const uint8_t *sfb, void *c, int out_dtype, int64_t M, int64_t N, int64_t K, void *stream);
+
+/* Grouped: forms 0 and 1 multiply the rows of group g (of A's M rows) by B[g]
+ * ([groups, N, K] or [groups, K, N], scale buffers group after group); rows of
+ * no group are set to zero if zero_tail, else left as they are.  Form 2 sums
+ * over each group's rows (K rows in all, operands and scales in slot order) into
+ * C [groups, M, N]; empty groups give zeros. */
+int ls_fp8_gemm_grouped(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t ldb, const uint8_t *sfa,
+                        const uint8_t *sfb, void *c, int out_dtype, int64_t M, int64_t N, int64_t K,
+                        const int *offsets, int64_t groups, int zero_tail, void *stream);
+
+/* For measurements and tests: 0 = choose by size (default); 1, 3, 4 = one CTA
+ * per tile with 128, 64 (form 0 only, else 128), 256 columns; 2 = CTA pairs. */
+int ls_fp8_gemm_set_variant(int variant);
+
 #ifdef __cplusplus
 }
 #endif

@@ -70,6 +70,16 @@ _SIGS = {
     "ls_wire_poll_status": (c_int, [c_vp, c_vp]),
     "ls_wire_reset": (c_int, [c_vp]),
     "ls_wire_debug_slots": (c_int, [c_vp, c_int, c_vp, ctypes.POINTER(c_i64), c_vp]),
+    "ls_fp8_sf_bytes": (c_i64, [c_i64, c_i64]),
+    "ls_fp8_slots": (c_i64, [c_i64, c_i64]),
+    "ls_quantize_fp8": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp]),
+    "ls_quantize_fp8_both": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_i64, c_vp]),
+    "ls_quantize_fp8_weight": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp]),
+    "ls_dequantize_fp8": (c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_int, c_vp, c_int, c_vp]),
+    "ls_fp8_gemm": (c_int, [c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_vp]),
+    "ls_fp8_gemm_grouped": (c_int, [c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64,
+                                    c_vp, c_i64, c_int, c_vp]),
+    "ls_fp8_gemm_set_variant": (c_int, [c_int]),
     "ls_scales_to_sf": (c_int, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "ls_scales_to_sf_block": (c_int, [c_vp, c_i64, c_i64, c_int, c_vp, c_vp, c_vp]),
     "ls_scales_to_sf_t": (c_int, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
@@ -111,6 +121,16 @@ def need_cuda(*tensors):
         if t is not None and not t.is_cuda:
             raise RuntimeError("lockstep_b200 computes on CUDA tensors only; got a "
                                f"{t.device.type} tensor (there is no CPU fallback)")
+
+
+def on_device_of(first, *others):
+    """Context that makes the tensors' device the current one; raises unless all of them (None
+    aside) are CUDA tensors of one device."""
+    need_cuda(first, *others)
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"lockstep_b200: tensors on different devices ({first.device} and {t.device})")
+    return torch.cuda.device(first.device)
 
 
 def aligned(t, n=16):

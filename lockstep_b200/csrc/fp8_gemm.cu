@@ -1,0 +1,556 @@
+// FP8 products with one scale per block of 128, dense and grouped by ragged row groups, on the
+// 5th-generation tensor cores (kind::mxf8f6f4, E4M3 operands, fp32 accumulators in tensor memory).
+//
+// The block scales are powers of two (UE8M0 bytes), so the tensor core applies them itself: an
+// MMA covers 32 values of K and takes one scale byte per row, the four MMAs of a block of 128
+// name the same byte.  One 512-byte scale tile (128 rows x 4 blocks) lasts 512 values of K, so
+// the scale copies cost a quarter of what they cost the MXFP4 product.
+//
+// Three forms of one kernel (A is the operand of the output's rows, B of its columns):
+//   NT  C = A[M, K] B[N, K]^T      forward                      A, B K-major
+//   NN  C = A[M, K] B[K, N]        gradient of the input        B MN-major
+//   TN  C = A[K, M]^T B[K, N]      gradient of the weight       A, B MN-major
+// so every operand is read as the quantizers wrote it; nothing is transposed in memory.
+// Grouped: NT and NN cut A's rows by `offsets` and take B[g]; TN cuts K (rows in slot order, see
+// fp8.cuh) and writes C[g].
+//
+// Roles of a CTA: warp 0 TMA producer, warp 1 MMA issuer, warps 2-9 epilogue.  CTAS = 2: a pair
+// of CTAs works on 256 x 256 tiles with cta_group::2 MMAs, each staging its own 128 rows of A and
+// its own half of B.  The tiles are handed out statically to a persistent grid.
+#include <cuda.h>
+#include <algorithm>
+#include <atomic>
+
+#include "epilogue.cuh"
+#include "fp8.cuh"
+#include "ptx.cuh"
+
+namespace ls {
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kTmemCols = 512;
+constexpr int kBlock = 128;             // values of K per stage = per scale block
+enum Form { NT = 0, NN = 1, TN = 2 };
+
+template <int CTAS, int BN>
+struct Fp8Cfg {
+    static_assert(CTAS == 1 || BN == 256, "pairs work on 256-column tiles");
+    static constexpr int BCOLS = BN / CTAS;                // columns of B staged by one CTA
+    static constexpr int A_BYTES = 128 * kBlock;
+    static constexpr int B_BYTES = BCOLS * kBlock;
+    static constexpr int SFB_TILES = BN >= 128 ? BN / 128 : 1;
+    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + 2048;       // 512 B of A's scales, 512 SFB_TILES of B's
+    static constexpr int STAGES = BN == 64 ? 8 : CTAS == 2 || BN == 128 ? 6 : 4;
+    static constexpr int OVL = BN == 256 ? 32 : 0;         // columns that the two accumulators share
+    static constexpr int ACC1 = BN - OVL;
+    static constexpr int SFA_COL = 2 * BN - OVL, SFB_COL = SFA_COL + 4;
+    static_assert(SFB_COL + 4 * SFB_TILES <= kTmemCols, "tensor memory overflow");
+    static constexpr int TAIL = STAGES * STAGE_BYTES;      // barriers, then offsets and tile prefix of the groups
+    static constexpr int LIST = TAIL + 256;
+    static constexpr int SMEM = LIST + 2 * 4 * (kFp8MaxGroups + 2) + 1024;
+    static_assert(SMEM <= 227 * 1024, "shared memory overflow");
+};
+
+struct Fp8Params {
+    void *c;
+    int M, N, K;                   // of the whole product: M counts the rows of all groups (NT, NN), K those of TN
+    int out_bf16;
+    const int *offsets;            // NULL: one group
+    int groups;
+    int zero_tail;                 // NT, NN: rows that belong to no group are set to zero
+    int sfa_kt, sfb_kt;            // scale tiles along K per 128 rows of A / columns of B
+    int sfb_rt;                    // NT, NN: 128-column scale tiles of one group's B
+    int *err;
+};
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_ctarank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+// One output tile of the CTA (pair): everything the three roles need.
+struct Item {
+    int g;                         // group
+    int row0, row_end;             // this CTA's first output row, and the end of the rows it may store
+    int n0;                        // first output column
+    int kb0, nkb;                  // blocks of K: scale index of the first, count
+    int slot;                      // this CTA's row tile in A's scale buffer
+};
+
+template <int CTAS, int BN, int FORM>
+__global__ void __launch_bounds__(kThreads, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb, const Fp8Params p)
+{
+    using C = Fp8Cfg<CTAS, BN>;
+    constexpr bool A_MN = FORM == TN, B_MN = FORM != NT;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *gen_base = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+    const uint32_t bar_base = smem_base + C::TAIL;
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (C::STAGES + s); };
+    // One "full" barrier per accumulator: with accumulators that share nothing, two tiles can be
+    // finished while a slow epilogue warp still stores the one before them, and a single barrier
+    // would be two phases ahead of it.
+    const uint32_t acc_full_bar = bar_base + 8u * (2 * C::STAGES);
+    const uint32_t acc_free_bar = acc_full_bar + 16u;      // two of them when the accumulators share nothing
+    const uint32_t tmem_slot = acc_free_bar + 16u;
+    volatile uint32_t *tmem_slot_p = reinterpret_cast<volatile uint32_t *>(gen_base + C::TAIL + 8 * (2 * C::STAGES + 4));
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot_p + 1);
+    int *list_off = reinterpret_cast<int *>(gen_base + C::LIST);       // [groups + 1] clamped offsets
+    int *list_pre = list_off + kFp8MaxGroups + 2;                      // [groups + 1] tiles (of 128 CTAS rows) before a group
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t cta = CTAS == 2 ? cluster_ctarank() : 0u;
+    const int worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; s++) {
+            ptx::mbar_init(full_bar(s), 1);
+            ptx::mbar_init(empty_bar(s), 1);
+        }
+        ptx::mbar_init(acc_full_bar, 1);
+        ptx::mbar_init(acc_full_bar + 8u, 1);
+        ptx::mbar_init(acc_free_bar, 8 * CTAS);
+        ptx::mbar_init(acc_free_bar + 8u, 8 * CTAS);
+        *abort_flag = 0;
+        ptx::fence_mbar_init();
+        ptx::prefetch_tmap(&tm_a);
+        ptx::prefetch_tmap(&tm_b);
+        ptx::prefetch_tmap(&tm_sfa);
+        ptx::prefetch_tmap(&tm_sfb);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc<CTAS>(tmem_slot, kTmemCols);
+        ptx::tmem_relinquish<CTAS>();
+    }
+    // Programmatic dependent launch: the set-up so far may overlap the kernel before this one;
+    // nothing below may.  Every thread waits (rows of no group are stored without a load).
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp == 2 && p.offsets) {
+        const int rows = FORM == TN ? p.K : p.M;
+        int before = 0;
+        for (int g0 = 0; g0 < p.groups; g0 += 32) {
+            const int g = g0 + lane;
+            int lo = rows, hi = rows;
+            if (g < p.groups) lo = group_lo(p.offsets, g, rows), hi = group_hi(p.offsets, g, rows, lo);
+            const int own = (hi - lo + 128 * CTAS - 1) / (128 * CTAS);
+            int sum = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            if (g < p.groups) {
+                list_off[g] = lo;
+                list_pre[g] = before + sum - own;
+                if (g == p.groups - 1) list_off[p.groups] = hi, list_pre[p.groups] = before + sum;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+        }
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (CTAS == 2) cluster_sync();                          // both CTAs' barriers exist before any remote arrive
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot_p;
+
+    // ---- the list of tiles, the same for every role
+    const int m_tiles = FORM == TN || !p.offsets ? (p.M + 128 * CTAS - 1) / (128 * CTAS) : list_pre[p.groups];
+    const int n_tiles = (p.N + BN - 1) / BN;
+    const int items = m_tiles * n_tiles * (FORM == TN ? p.groups : 1);
+    auto item_of = [&](int t) {
+        Item it;
+        const int mt = t % m_tiles, rest = t / m_tiles;
+        it.n0 = (FORM == TN ? rest % n_tiles : rest) * BN;
+        if (FORM == TN) {
+            it.g = rest / n_tiles;
+            it.row0 = mt * 128 * CTAS + 128 * int(cta);
+            it.row_end = p.M;
+            it.slot = mt * CTAS + int(cta);
+            const int lo = p.offsets ? list_off[it.g] : 0;
+            const int hi = p.offsets ? group_hi(p.offsets, it.g, p.K, lo) : p.K;
+            it.kb0 = p.offsets ? lo / 128 + it.g : 0;
+            it.nkb = (hi - lo + kBlock - 1) / kBlock;
+        } else {
+            it.g = 0;
+            int lo = 0, hi = p.M, i = mt;
+            if (p.offsets) {
+                int a = 0, b = p.groups - 1;                // last group whose tiles start at or before mt and that has any
+                while (a < b) {
+                    const int m = (a + b + 1) >> 1;
+                    if (list_pre[m] <= mt) a = m;
+                    else b = m - 1;
+                }
+                it.g = a;
+                lo = list_off[a], hi = group_hi(p.offsets, a, p.M, lo), i = mt - list_pre[a];
+            }
+            it.row0 = lo + (i * CTAS + int(cta)) * 128;
+            it.row_end = hi;
+            it.slot = (p.offsets ? lo / 128 + it.g : 0) + i * CTAS + int(cta);
+            it.kb0 = 0;
+            it.nkb = (p.K + kBlock - 1) / kBlock;
+        }
+        return it;
+    };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer (every CTA)
+        if (ptx::elect_one()) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int t = worker; t < items && ok; t += workers) {
+                const Item it = item_of(t);
+                const int sfb0 = (FORM == TN ? 0 : it.g * p.sfb_rt) + it.n0 / 128;
+                for (int k = 0; k < it.nkb; k++) {
+                    if (!(ok = ptx::mbar_wait(empty_bar(s), ph ^ 1, abort_flag))) break;
+                    const int kb = it.kb0 + k;
+                    const bool scales = k == 0 || (kb & 3) == 0;        // a scale tile lasts four blocks
+                    const uint32_t st = smem_base + s * C::STAGE_BYTES;
+                    // CTAS = 2: every load of either CTA completes on CTA 0's barrier
+                    const uint32_t bar = CTAS == 2 ? ptx::map_to_cta(full_bar(s), 0) : full_bar(s);
+                    if (cta == 0)
+                        ptx::mbar_expect_tx(full_bar(s), CTAS * (C::A_BYTES + C::B_BYTES + (scales ? 512u * (1 + C::SFB_TILES) : 0u)));
+                    if (A_MN) ptx::tma_load_3d<CTAS>(st, &tm_a, it.row0, kb * kBlock, 0, bar);
+                    else ptx::tma_load_3d<CTAS>(st, &tm_a, k * kBlock, it.row0, 0, bar);
+                    const uint32_t stb = st + C::A_BYTES;
+                    const int nb0 = it.n0 + int(cta) * C::BCOLS;
+#pragma unroll
+                    for (int b = 0; b < (C::BCOLS + 127) / 128; b++) {
+                        if (!B_MN) ptx::tma_load_3d<CTAS>(stb + b * 128 * kBlock, &tm_b, k * kBlock, nb0 + 128 * b, it.g, bar);
+                        else if (FORM == NN) ptx::tma_load_3d<CTAS>(stb + b * 128 * kBlock, &tm_b, nb0 + 128 * b, k * kBlock, it.g, bar);
+                        else ptx::tma_load_3d<CTAS>(stb + b * 128 * kBlock, &tm_b, nb0 + 128 * b, kb * kBlock, 0, bar);
+                    }
+                    if (scales) {
+                        const uint32_t stf = stb + C::B_BYTES;
+                        ptx::tma_load_3d<CTAS>(stf, &tm_sfa, 0, it.slot * p.sfa_kt + (kb >> 2), 0, bar);
+#pragma unroll
+                        for (int b = 0; b < C::SFB_TILES; b++)
+                            ptx::tma_load_3d<CTAS>(stf + 512 * (1 + b), &tm_sfb, 0, (sfb0 + b) * p.sfb_kt + (kb >> 2), 0, bar);
+                    }
+                    if (++s == C::STAGES) s = 0, ph ^= 1;
+                }
+            }
+            for (int i = 0; i < C::STAGES && ok; i++) {     // wait until the MMA side is done with every stage
+                ok = ptx::mbar_wait(empty_bar(s), ph ^ 1, abort_flag);
+                if (++s == C::STAGES) s = 0, ph ^= 1;
+            }
+        }
+    } else if (warp == 1 && cta == 0) {
+        // ------------------------------------------------------------ MMA issuer (CTA 0 of a pair)
+        if (ptx::elect_one()) {
+            constexpr uint32_t idesc = ptx::idesc_mxf8(128 * CTAS, BN, A_MN, B_MN);
+            const uint64_t adesc0 = A_MN ? ptx::desc_sw128_mn(smem_base, 128 * kBlock) : ptx::desc_sw128(smem_base);
+            const uint64_t bdesc0 = B_MN ? ptx::desc_sw128_mn(smem_base + C::A_BYTES, 128 * kBlock) : ptx::desc_sw128(smem_base + C::A_BYTES);
+            const uint64_t sfdesc0 = ptx::desc_sf(smem_base + C::A_BYTES + C::B_BYTES);
+            constexpr uint32_t A_STEP = A_MN ? 32 * 128 / 16 : 2, B_STEP = B_MN ? 32 * 128 / 16 : 2;   // 32 values of K
+            const uint32_t sfa_t = tmem_base + C::SFA_COL, sfb_t = tmem_base + C::SFB_COL;
+            int s = 0, lt = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int t = worker; t < items && ok; t += workers) {
+                const Item it = item_of(t);
+                if (it.nkb == 0) continue;                  // an empty group's weight gradient: no sum to take
+                if (C::OVL > 0) {
+                    // the tile before this one has been read out of the columns the two accumulators share
+                    if (lt > 0 && !(ok = ptx::mbar_wait(acc_free_bar, (lt - 1) & 1, abort_flag))) break;
+                } else {
+                    // this accumulator's previous tile (two tiles back) has been read out
+                    if (lt > 1 && !(ok = ptx::mbar_wait(acc_free_bar + 8u * (lt & 1), ((lt >> 1) - 1) & 1, abort_flag))) break;
+                }
+                ptx::tc_fence_after();
+                const uint32_t acc = tmem_base + ((lt & 1) ? C::ACC1 : 0);
+                // a 64-column tile uses one half of a 128-row scale tile: rows 32 c .. + 31 sit in column c
+                const uint32_t sfb_sub = BN >= 128 ? 0u : uint32_t(it.n0 & 127) / 32u;
+                for (int k = 0; k < it.nkb; k++) {
+                    if (!(ok = ptx::mbar_wait(full_bar(s), ph, abort_flag))) break;
+                    ptx::tc_fence_after();
+                    const int kb = it.kb0 + k;
+                    const uint32_t st16 = uint32_t(s) * (C::STAGE_BYTES >> 4);
+                    if (k == 0 || (kb & 3) == 0) {
+#pragma unroll
+                        for (int b = 0; b < 1 + C::SFB_TILES; b++) ptx::tmem_cp_sf<CTAS>(sfa_t + 4 * b, sfdesc0 + st16 + 32 * b);
+                    }
+                    const uint32_t id = uint32_t(kb & 3);   // byte of the scale column
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        ptx::mma_mxf8<CTAS>(acc, adesc0 + st16 + A_STEP * j, bdesc0 + st16 + B_STEP * j, idesc | (id << 29) | (id << 4),
+                                            sfa_t + (id << 30), sfb_t + sfb_sub + (id << 30), (k == 0 && j == 0) ? 0u : 1u);
+                    if (CTAS == 2) ptx::tc_commit_pair(empty_bar(s), 3);
+                    else ptx::tc_commit(empty_bar(s));
+                    if (++s == C::STAGES) s = 0, ph ^= 1;
+                }
+                if (ok) {
+                    if (CTAS == 2) ptx::tc_commit_pair(acc_full_bar + 8u * (lt & 1), 3);
+                    else ptx::tc_commit(acc_full_bar + 8u * (lt & 1));
+                }
+                lt++;
+            }
+        }
+    } else if (warp >= 2) {
+        // ------------------------------------------------------------ epilogue (every CTA)
+        // Warp w reads the tensor-memory lanes of quarter w % 4 and one half of the tile's columns.
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        const bool bf16 = p.out_bf16 != 0;
+        int lt = 0;
+        bool ok = true;
+        for (int t = worker; t < items && ok; t += workers) {
+            const Item it = item_of(t);
+            constexpr int CH = BN / 64;                     // chunks of 32 columns per warp
+            uint8_t *dst = static_cast<uint8_t *>(p.c) + (FORM == TN ? int64_t(it.g) * p.M * p.N * (bf16 ? 2 : 4) : 0);
+            const int row = it.row0 + 32 * q;
+            if (it.nkb == 0) {
+                uint32_t z[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) z[i] = 0u;
+#pragma unroll 1
+                for (int i = 0; i < CH; i++) store_chunk(it.row_end, p.N, dst, bf16, row, lane, it.n0 + 32 * (CH * half + i), z);
+                continue;
+            }
+            if (!(ok = ptx::mbar_wait(acc_full_bar + 8u * (lt & 1), (lt >> 1) & 1, abort_flag))) break;
+            ptx::tc_fence_after();
+            const uint32_t acc = tmem_base + ((lt & 1) ? C::ACC1 : 0) + (uint32_t(32 * q) << 16);
+            // The 32 columns shared by the accumulators are the last chunk of accumulator 0 and the
+            // first of accumulator 1: their owners read them first and then let the next tile's MMAs
+            // start; the other warps do so at once.  Without shared columns a warp frees its
+            // accumulator when its last load has landed.
+            const bool owner = C::OVL > 0 && ((lt & 1) ? half == 0 : half == 1);
+            const int start = (owner && !(lt & 1)) ? CH - 1 : 0;
+            auto chunk = [&](int i) { return CH * half + (C::OVL > 0 ? ((start + i) & (CH - 1)) : i); };
+            auto release = [&]() {
+                ptx::tc_fence_before();
+                __syncwarp();
+                const uint32_t bar = acc_free_bar + (C::OVL > 0 ? 0u : 8u * (lt & 1));
+                if (lane == 0) {
+                    if (CTAS == 2) ptx::mbar_arrive_cluster(bar, 0);
+                    else ptx::mbar_arrive(bar);
+                }
+            };
+            if (C::OVL > 0 && !owner) release();
+            uint32_t ra[32], rb[32];                        // the next chunk's load is in flight while this one is stored
+            ptx::tmem_ld32(acc + 32 * chunk(0), ra);
+#pragma unroll 1
+            for (int i = 0; i < CH; i += 2) {
+                ptx::tmem_ld_wait(ra);
+                if (i + 1 < CH) ptx::tmem_ld32(acc + 32 * chunk(i + 1), rb);
+                else if (C::OVL == 0) release();
+                if (i == 0 && owner) release();
+                store_chunk(it.row_end, p.N, dst, bf16, row, lane, it.n0 + 32 * chunk(i), ra);
+                if (i + 1 < CH) {
+                    ptx::tmem_ld_wait(rb);
+                    if (i + 2 < CH) ptx::tmem_ld32(acc + 32 * chunk(i + 2), ra);
+                    else if (C::OVL == 0) release();
+                    store_chunk(it.row_end, p.N, dst, bf16, row, lane, it.n0 + 32 * chunk(i + 1), rb);
+                }
+            }
+            lt++;
+        }
+        if (FORM != TN && p.offsets && p.zero_tail) {       // rows behind the last group
+            const int64_t bytes = int64_t(p.N) * (bf16 ? 2 : 4);
+            uint8_t *dst = static_cast<uint8_t *>(p.c);
+            const int first = group_hi(p.offsets, p.groups - 1, p.M, list_off[p.groups - 1]);
+            for (int r = first + blockIdx.x * 8 + warp - 2; r < p.M; r += gridDim.x * 8) {
+                uint8_t *line = dst + r * bytes;
+                if (bytes % 16 == 0)
+                    for (int64_t i = lane; i < bytes / 16; i += 32) reinterpret_cast<uint4 *>(line)[i] = make_uint4(0, 0, 0, 0);
+                else
+                    for (int64_t i = lane; i < bytes / 2; i += 32) reinterpret_cast<uint16_t *>(line)[i] = 0;
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    if (*abort_flag) {
+        for (int i = 0; i < 4096; i++) __nanosleep(256);    // copies and MMAs in flight land before memory is released
+        if (threadIdx.x == 0) atomicExch(p.err, 1);
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (CTAS == 2) cluster_sync();                          // neither CTA leaves while the other may still signal it
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc<CTAS>(tmem_base, kTmemCols);
+    }
+}
+
+// ---- host ---------------------------------------------------------------------
+struct MapSpec {
+    const void *base;
+    int64_t inner, rows, depth;    // bytes (u8) or words (scales), rows, matrices
+    int64_t pitch;                 // bytes between rows
+    int box_inner, box_rows;
+    bool scales;
+    bool operator==(const MapSpec &o) const
+    {
+        return base == o.base && inner == o.inner && rows == o.rows && depth == o.depth && pitch == o.pitch &&
+               box_inner == o.box_inner && box_rows == o.box_rows && scales == o.scales;
+    }
+};
+
+// Encoded tensor maps are pure functions of their specification: a direct-mapped cache per host
+// thread saves the driver's encoding for operands that come back (weights, recycled buffers).
+int make_map(CUtensorMap *m, const MapSpec &k)
+{
+    struct Slot { MapSpec key; CUtensorMap map; bool used; };
+    static thread_local Slot slots[256] = {};
+    uint64_t h = (reinterpret_cast<uintptr_t>(k.base) >> 4) ^ uint64_t(k.rows) * 0x9E3779B97F4A7C15ull ^
+                 uint64_t(k.inner) * 0xC2B2AE3D27D4EB4Full ^ uint64_t(k.depth * 131 + k.pitch * 31 + k.box_rows * 7 + k.scales);
+    h ^= h >> 29;
+    Slot &slot = slots[h % 256];
+    if (!slot.used || !(slot.key == k)) {
+        if (int rc = encode_map_3d(&slot.map, k.base, k.inner, k.rows, k.depth, k.pitch, k.box_inner, k.box_rows, k.scales)) {
+            slot.used = false;
+            return rc;
+        }
+        slot.key = k, slot.used = true;
+    }
+    *m = slot.map;
+    return LS_OK;
+}
+
+template <int CTAS, int BN, int FORM>
+int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa, const CUtensorMap &tsb, const Fp8Params &p,
+           int64_t most_tiles, cudaStream_t st)
+{
+    using C = Fp8Cfg<CTAS, BN>;
+    static int resident[64] = {};                           // CTAs (pairs) of this kernel that fit at once, per device
+    int dev = 0;
+    if (int rc = current_device(&dev)) return rc;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = CTAS, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    std::unique_lock<std::mutex> lk(state_mutex());
+    if (!resident[dev]) {
+        LS_CUDA(cudaFuncSetAttribute(fp8_gemm_kernel<CTAS, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        int n = sm_count();
+        if (CTAS == 2) {
+            cfg.gridDim = dim3(unsigned(sm_count() & ~1), 1, 1);
+            cfg.attrs = at + 1, cfg.numAttrs = 1;
+            LS_CUDA(cudaOccupancyMaxActiveClusters(&n, fp8_gemm_kernel<CTAS, BN, FORM>, &cfg));
+            if (n < 1) return fail(LS_ECUDA, "no CTA pair of the FP8 product fits on this device");
+        }
+        resident[dev] = n;
+    }
+    const int64_t workers = std::max<int64_t>(1, std::min<int64_t>(most_tiles, resident[dev]));
+    lk.unlock();
+    cfg.gridDim = dim3(unsigned(CTAS * workers), 1, 1);
+    cfg.attrs = at, cfg.numAttrs = CTAS == 2 ? 2 : 1;
+    LS_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<CTAS, BN, FORM>, ta, tb, tsa, tsb, p));
+    return LS_OK;
+}
+
+std::atomic<int> g_variant{0};          // 0 = choose by size; 1 / 2 = single CTA (128 columns) / CTA pair; 3, 4 = single CTA with 64, 256 columns
+
+int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t ldb, const uint8_t *sfa, const uint8_t *sfb,
+             void *c, int out_dtype, int64_t M, int64_t N, int64_t K, const int *offsets, int64_t groups, int zero_tail,
+             void *stream)
+{
+    if (int rc = check_device()) return rc;
+    if (form < NT || form > TN) return fail(LS_EINVAL, "form must be 0 (NT), 1 (NN) or 2 (TN)");
+    if (out_dtype != LS_F32 && out_dtype != LS_BF16) return fail(LS_EINVAL, "unsupported output dtype %d", out_dtype);
+    if (M < 0 || N < 0 || K < 0 || M > (1 << 30) || N > (1 << 30) || K > (1 << 30)) return fail(LS_EINVAL, "dimension out of range");
+    if (groups < 1 || groups > kFp8MaxGroups) return fail(LS_EINVAL, "groups=%lld must be 1..%d", (long long)groups, kFp8MaxGroups);
+    if (groups > 1 && !offsets) return fail(LS_EINVAL, "several groups need offsets");
+    if (M == 0 || N == 0) return LS_OK;
+    if (!c) return fail(LS_EINVAL, "null pointer");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (K == 0) {                                           // empty sums
+        LS_CUDA(cudaMemsetAsync(c, 0, size_t(form == TN ? groups : 1) * M * N * (out_dtype == LS_BF16 ? 2 : 4), st));
+        return LS_OK;
+    }
+    if (!a || !b || !sfa || !sfb) return fail(LS_EINVAL, "null pointer");
+    if (!aligned16(a) || !aligned16(b) || !aligned16(sfa) || !aligned16(sfb) || !aligned16(c))
+        return fail(LS_EALIGN, "operands, scale buffers and outputs must be 16-byte aligned");
+    const int64_t a_inner = form == TN ? M : K, b_inner = form == NT ? K : N;
+    if (lda < a_inner || ldb < b_inner || lda % 16 || ldb % 16)
+        return fail(LS_EINVAL, "row pitches must be multiples of 16 and cover a row (lda=%lld, ldb=%lld)", (long long)lda, (long long)ldb);
+    int *err = error_word();
+    if (!err) return fail(LS_ECUDA, "could not allocate the device error word");
+
+    // Rows (M) or K that the operands hold: with groups the TN operands are in slot order.
+    const int64_t slots = offsets ? fp8_slots(form == TN ? K : M, groups) : ((form == TN ? K : M) + 127) / 128;
+    const int64_t a_rows = form == TN ? (offsets ? slots * 128 : K) : M;
+    const int64_t b_rows = form == NT ? N : form == NN ? K : a_rows;
+    const int64_t depth = form == TN ? 1 : groups;
+    const int64_t kblocks = form == TN ? slots : (K + 127) / 128;
+    Fp8Params p{};
+    p.c = c, p.M = int(M), p.N = int(N), p.K = int(K);
+    p.out_bf16 = out_dtype == LS_BF16;
+    p.offsets = offsets, p.groups = int(groups), p.zero_tail = zero_tail;
+    p.sfa_kt = p.sfb_kt = int((kblocks + 3) / 4);
+    p.sfb_rt = int((N + 127) / 128);
+    p.err = err;
+
+    // Which kernel: see the note at choose() below.
+    const int variant = g_variant.load(std::memory_order_relaxed);
+    const int64_t rows_per_group = form == TN ? M : M / groups;
+    bool pair = variant ? variant == 2 : rows_per_group > 128;
+    int bn = 256;
+    if (!pair) {
+        bn = variant == 4 ? 256 : 128;
+        if (form == NT && (variant == 3 || (variant == 0 && ((M + 127) / 128 + groups - 1) * ((N + 127) / 128) * 2 <= sm_count()))) bn = 64;
+    }
+    const int64_t tile_rows = pair ? 256 : 128;
+    const int64_t m_tiles = form == TN || !offsets ? (M + tile_rows - 1) / tile_rows : M / tile_rows + groups;
+    const int64_t items = m_tiles * ((N + bn - 1) / bn) * (form == TN ? groups : 1);
+    if (items > 0x7FFFFFFFll) return fail(LS_EINVAL, "too many output tiles");
+    const int64_t a_tiles = fp8_sf_tiles(form == TN ? M : slots * 128, kblocks);
+    const int64_t b_tiles = fp8_sf_tiles(N, kblocks) * depth;
+    CUtensorMap ta, tb, tsa, tsb;
+    if (int rc = make_map(&ta, {a, a_inner, a_rows, 1, lda, 128, 128, false})) return rc;
+    if (int rc = make_map(&tb, {b, b_inner, b_rows, depth, ldb, 128, form == NT && bn == 64 ? 64 : 128, false})) return rc;
+    if (int rc = make_map(&tsa, {sfa, 128, a_tiles, 1, 512, 128, 1, true})) return rc;
+    if (int rc = make_map(&tsb, {sfb, 128, b_tiles, 1, 512, 128, 1, true})) return rc;
+#define LS_FP8_LAUNCH(F)                                                                        \
+    if (form == F) return pair ? launch<2, 256, F>(ta, tb, tsa, tsb, p, items, st)              \
+                        : bn == 256 ? launch<1, 256, F>(ta, tb, tsa, tsb, p, items, st)         \
+                                    : launch<1, 128, F>(ta, tb, tsa, tsb, p, items, st);
+    if (form == NT && bn == 64) return launch<1, 64, NT>(ta, tb, tsa, tsb, p, items, st);
+    LS_FP8_LAUNCH(NT)
+    LS_FP8_LAUNCH(NN)
+    LS_FP8_LAUNCH(TN)
+#undef LS_FP8_LAUNCH
+    return LS_OK;
+}
+
+}  // namespace
+}  // namespace ls
+
+using namespace ls;
+
+extern "C" int ls_fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t ldb, const uint8_t *sfa,
+                           const uint8_t *sfb, void *c, int out_dtype, int64_t M, int64_t N, int64_t K, void *stream)
+{
+    return fp8_gemm(form, a, lda, b, ldb, sfa, sfb, c, out_dtype, M, N, K, nullptr, 1, 0, stream);
+}
+
+extern "C" int ls_fp8_gemm_grouped(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t ldb, const uint8_t *sfa,
+                                   const uint8_t *sfb, void *c, int out_dtype, int64_t M, int64_t N, int64_t K,
+                                   const int *offsets, int64_t groups, int zero_tail, void *stream)
+{
+    if (!offsets) return fail(LS_EINVAL, "null pointer");
+    return fp8_gemm(form, a, lda, b, ldb, sfa, sfb, c, out_dtype, M, N, K, offsets, groups, zero_tail, stream);
+}
+
+extern "C" int ls_fp8_gemm_set_variant(int variant)
+{
+    if (variant < 0 || variant > 4) return fail(LS_EINVAL, "variant must be 0..4");
+    g_variant.store(variant, std::memory_order_relaxed);
+    return LS_OK;
+}

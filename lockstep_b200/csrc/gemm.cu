@@ -22,6 +22,7 @@
 #include <cstdlib>
 
 #include "common.cuh"
+#include "epilogue.cuh"
 #include "ptx.cuh"
 
 namespace ls {
@@ -136,103 +137,6 @@ __device__ __forceinline__ void quant_chunk(const Epi &p, int row, int col0, con
     }
     *reinterpret_cast<uint4 *>(p.q_packed + int64_t(row) * (p.N / 2) + col0 / 2) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
     p.q_sf[sf_offset(uint32_t(row), uint32_t(col0 / 32), uint32_t(p.N / 128))] = uint8_t(e8);
-}
-
-// 4 x 4 transpose of 16-byte items inside each group of four lanes: afterwards item k of
-// lane 4g + j is what lane 4g + k held as item j.
-__device__ __forceinline__ void transpose4(uint4 (&it)[4], int lane)
-{
-#pragma unroll
-    for (int b = 0; b < 2; b++) {
-        const bool up = (lane >> b) & 1;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (i & (1 << b)) continue;
-            const int hi = i | (1 << b);
-            uint4 send = up ? it[i] : it[hi], recv;
-            recv.x = __shfl_xor_sync(0xFFFFFFFFu, send.x, 1 << b);
-            recv.y = __shfl_xor_sync(0xFFFFFFFFu, send.y, 1 << b);
-            recv.z = __shfl_xor_sync(0xFFFFFFFFu, send.z, 1 << b);
-            recv.w = __shfl_xor_sync(0xFFFFFFFFu, send.w, 1 << b);
-            if (up) it[i] = recv;
-            else it[hi] = recv;
-        }
-    }
-}
-
-// Ragged edge of the output (N not a multiple of the vector width, or the last columns of
-// a tile): element-wise stores from a private copy of the chunk.  Kept out of line, and fed
-// from a copy, so that neither its loop nor its run-time index touches the epilogue's
-// accumulator registers (a run-time index into them would move them to local memory) or
-// its code size (a tile's epilogue runs once per tile; short tiles pay for every
-// instruction fetched).
-__device__ __noinline__ void store_tail_impl(void *dst, bool bf16, int n, const uint32_t *v)
-{
-    if (bf16)
-        for (int j = 0; j < n; j++) static_cast<__nv_bfloat16 *>(dst)[j] = __float2bfloat16_rn(__uint_as_float(v[j]));
-    else
-        for (int j = 0; j < n; j++) static_cast<float *>(dst)[j] = __uint_as_float(v[j]);
-}
-__device__ __forceinline__ void store_tail(void *dst, bool bf16, int n, const uint32_t (&r)[32])
-{
-    uint32_t v[32];
-#pragma unroll
-    for (int j = 0; j < 32; j++) v[j] = r[j];
-    store_tail_impl(dst, bf16, n, v);
-}
-
-// Stores one accumulator chunk: lane l of the warp holds the 32 consecutive outputs
-// (columns col0 .. col0 + 31) of row row0 + l.  Called by the whole warp.  Storing each
-// lane's own row would touch 32 rows per instruction (one 16-byte piece each); the
-// pieces are transposed inside groups of four lanes first, so that four adjacent lanes
-// write 64 contiguous bytes of one row and an instruction touches 8 rows.
-__device__ __forceinline__ void store_chunk(const Epi &p, void *cbase, bool bf16, int row0, int lane, int col0,
-                                            const uint32_t (&r)[32])
-{
-    if (row0 >= p.M || col0 >= p.N) return;                       // uniform over the warp
-    const int row = row0 + lane;
-    const int trow = row0 + (lane & ~3), tq = lane & 3;            // first row / piece of this lane after a transpose
-    if (bf16) {
-        __nv_bfloat16 *base = static_cast<__nv_bfloat16 *>(cbase);
-        if (col0 + 32 <= p.N && (p.N & 7) == 0) {
-            uint4 it[4];
-#pragma unroll
-            for (int v = 0; v < 4; v++) {
-                uint32_t *ow = &it[v].x;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[8 * v + 2 * j]),
-                                                             __uint_as_float(r[8 * v + 2 * j + 1]));
-                    ow[j] = *reinterpret_cast<uint32_t *>(&h);
-                }
-            }
-            transpose4(it, lane);
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (trow + k < p.M)
-                    *reinterpret_cast<uint4 *>(base + int64_t(trow + k) * p.N + col0 + 8 * tq) = it[k];
-        } else if (row < p.M) {
-            store_tail(base + int64_t(row) * p.N + col0, true, min(32, p.N - col0), r);
-        }
-    } else {
-        float *base = static_cast<float *>(cbase);
-        if (col0 + 32 <= p.N && (p.N & 3) == 0) {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint4 it[4];
-#pragma unroll
-                for (int v = 0; v < 4; v++)
-                    it[v] = make_uint4(r[16 * h + 4 * v], r[16 * h + 4 * v + 1], r[16 * h + 4 * v + 2], r[16 * h + 4 * v + 3]);
-                transpose4(it, lane);
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (trow + k < p.M)
-                        *reinterpret_cast<uint4 *>(base + int64_t(trow + k) * p.N + col0 + 16 * h + 4 * tq) = it[k];
-            }
-        } else if (row < p.M) {
-            store_tail(base + int64_t(row) * p.N + col0, false, min(32, p.N - col0), r);
-        }
-    }
 }
 
 // One pipeline stage on the tensor pipe: scale tiles shared -> tensor memory, then the
@@ -452,7 +356,7 @@ mxfp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_consta
             const int first = (C::OVL && !(lt & 1)) ? CH - 1 : 0;
             // two register sets: the load of the next chunk is in flight while this one is stored
             auto emit = [&](int c, const uint32_t (&r)[32]) {
-                if (ep.store_c || splits > 1) store_chunk(ep, dst, dst_bf16, row - lane, lane, nt * BN + 32 * c, r);
+                if (ep.store_c || splits > 1) store_chunk(ep.M, ep.N, dst, dst_bf16, row - lane, lane, nt * BN + 32 * c, r);
                 if (ep.q_packed) quant_chunk(ep, row, nt * BN + 32 * c, r);
             };
             uint32_t ra[32], rb[32];
@@ -769,7 +673,7 @@ mxfp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a0, const __grid_c
             auto chunk = [&](int i) { return CH * half + (SH > 0 ? ((start + i) & (CH - 1)) : i); };
             if (SH > 0 && !owner) release_next_tile();
             auto emit = [&](int c, const uint32_t (&r)[32]) {
-                if (ep.store_c || splits > 1) store_chunk(ep, dst, dst_bf16, row - lane, lane, nt * C::BN + 32 * c, r);
+                if (ep.store_c || splits > 1) store_chunk(ep.M, ep.N, dst, dst_bf16, row - lane, lane, nt * C::BN + 32 * c, r);
                 if (ep.q_packed) quant_chunk(ep, row, nt * C::BN + 32 * c, r);
             };
             // two register sets: the load of the next chunk is in flight while this one is stored
@@ -1041,6 +945,23 @@ void splitk_release(cudaStream_t st)
 }
 
 }  // namespace
+
+int encode_map_3d(void *map, const void *base, int64_t inner, int64_t rows, int64_t depth, int64_t pitch, int box_inner,
+                  int box_rows, bool words)
+{
+    EncodeFn fn = encode_fn();
+    if (!fn) return fail(LS_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t dims[3] = {cuuint64_t(inner), cuuint64_t(rows), cuuint64_t(depth)};
+    cuuint64_t strides[2] = {cuuint64_t(pitch), cuuint64_t(pitch) * cuuint64_t(rows)};
+    cuuint32_t box[3] = {cuuint32_t(box_inner), cuuint32_t(box_rows), 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(static_cast<CUtensorMap *>(map), words ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3,
+                    const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    words ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(LS_ECUDA, "cuTensorMapEncodeTiled failed with %d", int(r));
+    return LS_OK;
+}
 
 int *error_word()
 {

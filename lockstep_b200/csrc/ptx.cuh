@@ -97,6 +97,18 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
                  " [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+template <int CTAS>
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *m, int x, int y, int z, uint32_t bar)
+{
+    if (CTAS == 1)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+                     " [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+                     " [%0], [%1, {%2, %3, %4}], [%5];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
 // linear copy global -> shared; addresses 16-byte aligned, size a multiple of 16
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
 {
@@ -166,6 +178,22 @@ __device__ __forceinline__ void mma_mxf4_block16(uint32_t d, uint64_t adesc, uin
                      ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb) : "memory");
 }
 
+// E4M3 operands, K = 32 per instruction, one UE8M0 scale byte per row (byte number in the
+// instruction descriptor and in the top bits of the scale address)
+template <int CTAS>
+__device__ __forceinline__ void mma_mxf8(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t sfa, uint32_t sfb, uint32_t accumulate)
+{
+    if (CTAS == 1)
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                     "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n}\n"
+                     ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb) : "memory");
+    else
+        asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                     "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n}\n"
+                     ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb) : "memory");
+}
+
 // arrive on a barrier of this CTA once every tcgen05 op issued so far by this thread is done
 __device__ __forceinline__ void tc_commit(uint32_t bar)
 {
@@ -211,6 +239,13 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t smem_addr)
     return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) |
            (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
+// MN-major operand tile of bytes with the 128-byte swizzle: a row holds 128 consecutive M (or N)
+// indices of one k, 8-k groups are 1024 bytes apart, the next 128 indices start `chunk` bytes on.
+__device__ __forceinline__ uint64_t desc_sw128_mn(uint32_t smem_addr, uint32_t chunk)
+{
+    return uint64_t((smem_addr & 0x3FFFFu) >> 4) | (uint64_t(chunk >> 4) << 16) | (uint64_t(1024 >> 4) << 32) |
+           (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
 // 32 rows x 16 bytes, unswizzled, 8-row groups 128 bytes apart (scale factors)
 __device__ __forceinline__ uint64_t desc_sf(uint32_t smem_addr)
 {
@@ -220,6 +255,12 @@ __device__ __forceinline__ uint64_t desc_sf(uint32_t smem_addr)
 __host__ __device__ constexpr uint32_t idesc_mxf4(int M, int N)
 {
     return (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (1u << 23) | (uint32_t(M >> 4) << 24);
+}
+
+// instruction descriptor: E4M3 x E4M3, UE8M0 scales, fp32 accumulate; major = 1: MN-major operand
+__host__ __device__ constexpr uint32_t idesc_mxf8(int M, int N, int a_mn, int b_mn)
+{
+    return (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) | (uint32_t(N >> 3) << 17) | (1u << 23) | (uint32_t(M >> 4) << 24);
 }
 
 }  // namespace ptx
