@@ -475,6 +475,28 @@ int ls_fp8_gemm_grouped(int form, const uint8_t *a, int64_t lda, const uint8_t *
                         const uint8_t *sfb, void *c, int out_dtype, int64_t M, int64_t N, int64_t K,
                         const int *offsets, int64_t groups, int zero_tail, void *stream);
 
+/* The linear layer in one call per direction, groups = 1 and offsets NULL for a
+ * dense one.  `work` and `saved` are buffers of ls_fp8_linear_bytes(what, ...)
+ * bytes (groups = 0: dense), 16-byte aligned; work may be reused once the call's
+ * kernels are done, saved goes from forward to backward.  grads: 1 = the
+ * gradient of x is wanted, 2 = of w (the same value in all calls of a layer).
+ *   ls_fp8_linear           y = x w^T for a weight quantized beforehand
+ *   ls_fp8_linear_forward   quantizes w too; y has x's type
+ *   ls_fp8_linear_backward  gx [rows, K], gw ([groups,] N, K) of gy [rows, N] */
+#define LS_FP8_SERVE    0   /* what: work of ls_fp8_linear */
+#define LS_FP8_FORWARD  1   /* work of ls_fp8_linear_forward */
+#define LS_FP8_SAVED    2
+#define LS_FP8_BACKWARD 3   /* work of ls_fp8_linear_backward */
+int64_t ls_fp8_linear_bytes(int what, int64_t rows, int64_t N, int64_t K, int64_t groups, int grads);
+int ls_fp8_linear(const void *x, int dtype, int64_t rows, int64_t K, const uint8_t *w_codes, int64_t ldw,
+                  const uint8_t *w_sf, int64_t N, void *y, int out_dtype, const int *offsets, int64_t groups,
+                  int zero_tail, void *work, void *stream);
+int ls_fp8_linear_forward(const void *x, int dtype, const void *w, int w_dtype, int64_t rows, int64_t N, int64_t K,
+                          const int *offsets, int64_t groups, int grads, void *y, void *saved, void *work, void *stream);
+int ls_fp8_linear_backward(const void *gy, int dtype, int64_t rows, int64_t N, int64_t K, const int *offsets,
+                           int64_t groups, int grads, const void *saved, void *gx, int gx_dtype, void *gw,
+                           int gw_dtype, void *work, void *stream);
+
 /* For measurements and tests: 0 = choose by size (default); 1, 3, 4 = one CTA
  * per tile with 128, 64 (form 0 only, else 128), 256 columns; 2 = CTA pairs. */
 int ls_fp8_gemm_set_variant(int variant);

@@ -4,6 +4,7 @@ There is no CPU path: if the shared object is missing, or a tensor is not on a
 CUDA device, the call raises.
 """
 
+import contextlib
 import ctypes
 from pathlib import Path
 
@@ -79,6 +80,11 @@ _SIGS = {
     "ls_fp8_gemm": (c_int, [c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64, c_vp]),
     "ls_fp8_gemm_grouped": (c_int, [c_int, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_int, c_i64, c_i64, c_i64,
                                     c_vp, c_i64, c_int, c_vp]),
+    "ls_fp8_linear_bytes": (c_i64, [c_int, c_i64, c_i64, c_i64, c_i64, c_int]),
+    "ls_fp8_linear": (c_int, [c_vp, c_int, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_int, c_vp, c_i64, c_int, c_vp, c_vp]),
+    "ls_fp8_linear_forward": (c_int, [c_vp, c_int, c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_int, c_vp, c_vp, c_vp, c_vp]),
+    "ls_fp8_linear_backward": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_vp, c_int,
+                                       c_vp, c_vp]),
     "ls_fp8_gemm_set_variant": (c_int, [c_int]),
     "ls_scales_to_sf": (c_int, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "ls_scales_to_sf_block": (c_int, [c_vp, c_i64, c_i64, c_int, c_vp, c_vp, c_vp]),
@@ -123,14 +129,20 @@ def need_cuda(*tensors):
                                f"{t.device.type} tensor (there is no CPU fallback)")
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device_of(first, *others):
     """Context that makes the tensors' device the current one; raises unless all of them (None
     aside) are CUDA tensors of one device."""
-    need_cuda(first, *others)
+    d = first.get_device()
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != d:
+            need_cuda(first, *others)
             raise RuntimeError(f"lockstep_b200: tensors on different devices ({first.device} and {t.device})")
-    return torch.cuda.device(first.device)
+    if d < 0:
+        need_cuda(first)
+    return _HERE if torch.cuda.current_device() == d else torch.cuda.device(d)
 
 
 def aligned(t, n=16):

@@ -14,55 +14,81 @@ namespace {
 
 constexpr uint32_t kAbs = 0x7FFFFFFFu;
 
-// bits of |v|, 0 for an infinity or a NaN
-__device__ __forceinline__ uint32_t finite_abs(float v)
+// Values are kept as the 32-bit words they were loaded in: one fp32 value, or two bf16 values.
+// bf16 pairs are handled two at a time: packed NaN-propagating maxima of magnitudes (a 16-bit
+// integer maximum of pairs is several instructions), and scaled by a packed multiplication, which is
+// exact (a power of two; results below bf16's range are far below E4M3's).
+template <typename T> struct Word {
+    static constexpr bool PAIR = sizeof(T) == 2;
+    static constexpr uint32_t MAG = PAIR ? 0x7FFF7FFFu : kAbs;
+    static __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b)   // of magnitudes
+    {
+        if constexpr (!PAIR) return max(a, b);
+        uint32_t m;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+        return m;
+    }
+    // fp32 bits of the larger half
+    static __device__ __forceinline__ uint32_t fold(uint32_t m) { return PAIR ? max(m & 0xFFFF0000u, m << 16) : m; }
+    // the reciprocal scale as a word that multiplies (both halves of) a word
+    static __device__ __forceinline__ uint32_t inv(uint32_t e8m0)
+    {
+        return PAIR ? ((254u - e8m0) << 7) * 0x00010001u : (254u - e8m0) << 23;
+    }
+    // E4M3 codes of two words of pairs, or four words, times their reciprocal scales
+    static __device__ __forceinline__ uint32_t codes(const uint32_t *w, const uint32_t *inv)
+    {
+        if constexpr (PAIR) {
+            uint32_t q[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(q[i]) : "r"(w[i]), "r"(inv[i]));
+            return cvt_e4m3x4(__uint_as_float(q[0] << 16), __uint_as_float(q[0] & 0xFFFF0000u),
+                              __uint_as_float(q[1] << 16), __uint_as_float(q[1] & 0xFFFF0000u));
+        } else {
+            return cvt_e4m3x4(__uint_as_float(w[0]) * __uint_as_float(inv[0]), __uint_as_float(w[1]) * __uint_as_float(inv[1]),
+                              __uint_as_float(w[2]) * __uint_as_float(inv[2]), __uint_as_float(w[3]) * __uint_as_float(inv[3]));
+        }
+    }
+    // sets a non-finite value to zero and flags it: bit 0 the low half (or the value), bit 1 the high half
+    static __device__ __forceinline__ uint32_t drop_special(uint32_t &w)
+    {
+        uint32_t flags = 0;
+        if constexpr (PAIR) {
+            if ((w & 0x7F80u) == 0x7F80u) flags |= 1u, w &= 0xFFFF0000u;
+            if ((w & 0x7F800000u) == 0x7F800000u) flags |= 2u, w &= 0xFFFFu;
+        } else if ((w & kAbs) >= kBitsInf) {
+            flags = 1u, w = 0u;
+        }
+        return flags;
+    }
+};
+
+// E4M3 has no infinity: non-finite values, whose codes were stored as zeros, become its NaN.
+// Byte stores out of line, so that the ordinary path carries none of it.
+__device__ __noinline__ void store_nans(uint8_t *dst, uint32_t flags)
 {
-    const uint32_t a = __float_as_uint(v) & kAbs;
-    return a < kBitsInf ? a : 0u;
-}
-// E4M3 has no infinity: both kinds of non-finite value are stored as its NaN
-__device__ __forceinline__ float finite_or_nan(float v)
-{
-    return (__float_as_uint(v) & kAbs) < kBitsInf ? v : __uint_as_float(0x7FC00000u);
+    for (; flags; flags &= flags - 1) dst[__ffs(flags) - 1] = 0x7F;
 }
 
-// N consecutive values from x[0 .. N), of which the first `left` exist (zeros after them).
-template <int N, bool VEC, typename T>
-__device__ __forceinline__ void load_values(const T *x, int left, float (&v)[N])
+// 32 bytes in one instruction: two 16-byte loads of a lane would fetch every 32-byte sector twice
+__device__ __forceinline__ void ld_stream32(const void *p, uint32_t *w)
 {
-    if constexpr (VEC) {
-        if (left <= 0) {
+    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+}
+
+// WORDS words of consecutive values from x, of which the first `left` values exist (zeros after them)
+template <int WORDS, typename T>
+__device__ __forceinline__ void load_ragged(const T *x, int left, uint32_t *w)
+{
 #pragma unroll
-            for (int i = 0; i < N; i++) v[i] = 0.0f;
-            return;
-        }
+    for (int i = 0; i < WORDS; i++) {
         if constexpr (sizeof(T) == 2) {
-#pragma unroll
-            for (int h = 0; h < N / 8; h++) {
-                const uint4 u = ld_stream(reinterpret_cast<const uint4 *>(x) + h);
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    v[8 * h + 2 * i] = __uint_as_float(w[i] << 16);
-                    v[8 * h + 2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-                }
-            }
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(x);
+            const uint32_t lo = 2 * i < left ? h[2 * i] : 0u, hi = 2 * i + 1 < left ? h[2 * i + 1] : 0u;
+            w[i] = lo | (hi << 16);
         } else {
-#pragma unroll
-            for (int h = 0; h < N / 4; h++) {
-                const uint4 u = ld_stream(reinterpret_cast<const uint4 *>(x) + h);
-                v[4 * h] = __uint_as_float(u.x), v[4 * h + 1] = __uint_as_float(u.y);
-                v[4 * h + 2] = __uint_as_float(u.z), v[4 * h + 3] = __uint_as_float(u.w);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            v[i] = 0.0f;
-            if (i < left) {
-                if constexpr (sizeof(T) == 2) v[i] = __bfloat162float(x[i]);
-                else v[i] = x[i];
-            }
+            w[i] = i < left ? __float_as_uint(x[i]) : 0u;
         }
     }
 }
@@ -70,53 +96,108 @@ __device__ __forceinline__ void load_values(const T *x, int left, float (&v)[N])
 // ---- blocks along the rows of a dense tensor -----------------------------------------------
 // One warp takes 512 consecutive values of a row = 4 blocks = one scale word; 8 lanes share a block.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
+__device__ __forceinline__ void load_chunk(const T *x, int left, uint32_t (&w)[8 * sizeof(T) / 2])
+{
+    constexpr int WORDS = 8 * sizeof(T) / 2;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int h = 0; h < WORDS / 8; h++) {
+            if (left > 0) ld_stream32(x + 32 / int(sizeof(T)) * h, w + 8 * h);
+            else
+                for (int i = 0; i < 8; i++) w[8 * h + i] = 0u;
+        }
+    } else {
+        load_ragged<WORDS>(x, left, w);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void quantize_chunk(uint32_t (&w)[8 * sizeof(T) / 2], int64_t row, int chunk, int K, int chunks,
+                                               uint8_t *codes, int64_t ld, float *scale, uint8_t *sf)
+{
+    using W = Word<T>;
+    constexpr int WORDS = 8 * sizeof(T) / 2, PER = WORDS / 4;
+    const int lane = threadIdx.x & 31, col = chunk * 512 + lane * 16;
+    auto largest = [&]() {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) m = W::max_of(m, w[i] & W::MAG);
+        return W::fold(m);
+    };
+    uint32_t amax = largest(), flags = 0;
+    const bool special = __any_sync(0xFFFFFFFFu, amax >= kBitsInf);
+    if (special) {
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) flags |= W::drop_special(w[i]) << (i * 16 / WORDS);
+        amax = largest();
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+    const uint32_t e8 = fp8_e8m0(amax), s = W::inv(e8);
+    if (col < K) {
+        const uint32_t inv[4] = {s, s, s, s};
+        uint32_t c[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) c[j] = W::codes(w + PER * j, inv);
+        *reinterpret_cast<uint4 *>(codes + row * ld + col) = make_uint4(c[0], c[1], c[2], c[3]);
+        if (special) store_nans(codes + row * ld + col, flags);
+        if (scale && (lane & 7) == 0) scale[row * ((K + 127) / 128) + col / 128] = __uint_as_float(e8 << 23);
+    }
+    if (sf) {
+        // the four blocks' bytes as one word: lanes 0, 8, 16, 24 put theirs in place
+        const uint32_t word = __reduce_or_sync(0xFFFFFFFFu, e8 << (lane & 24));
+        if (lane == 0)
+            *reinterpret_cast<uint32_t *>(sf + sf_offset(uint32_t(row), uint32_t(chunk * 4), uint32_t(chunks))) = word;
+    }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256, 4)
 fp8_rows_kernel(const T *__restrict__ x, int64_t rows, int K, uint8_t *__restrict__ codes, int64_t ld,
                 float *__restrict__ scale, uint8_t *__restrict__ sf)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
-    const int chunks = (K + 511) / 512, blocks = (K + 127) / 128;
-    const int64_t total = rows * chunks, step = int64_t(gridDim.x) * 8;
-    for (int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); i < total; i += step) {
-        const int64_t row = i / chunks;
-        const int chunk = int(i - row * chunks), col = chunk * 512 + lane * 16;
-        float v[16];
-        load_values<16, VEC>(x + row * K + col, K - col, v);
-        uint32_t amax = 0;
-#pragma unroll
-        for (int j = 0; j < 16; j++) amax = max(amax, __float_as_uint(v[j]) & kAbs);
-        if (__any_sync(0xFFFFFFFFu, amax >= kBitsInf)) {
-            amax = 0;
-#pragma unroll
-            for (int j = 0; j < 16; j++) amax = max(amax, finite_abs(v[j])), v[j] = finite_or_nan(v[j]);
-        }
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-        const uint32_t e8 = fp8_e8m0(amax);
-        const float inv = fp8_inv_scale(e8);
-        if (col < K) {
-            uint32_t c[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                c[j] = cvt_e4m3x4(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
-            *reinterpret_cast<uint4 *>(codes + row * ld + col) = make_uint4(c[0], c[1], c[2], c[3]);
-        }
-        if (scale && (lane & 7) == 0 && col < K) scale[row * blocks + col / 128] = __uint_as_float(e8 << 23);
-        if (sf) {
-            const uint32_t b1 = __shfl_down_sync(0xFFFFFFFFu, e8, 8), b2 = __shfl_down_sync(0xFFFFFFFFu, e8, 16),
-                           b3 = __shfl_down_sync(0xFFFFFFFFu, e8, 24);
-            if (lane == 0)
-                *reinterpret_cast<uint32_t *>(sf + sf_offset(uint32_t(row), uint32_t(chunk * 4), uint32_t(chunks))) =
-                    e8 | (b1 << 8) | (b2 << 16) | (b3 << 24);
-        }
+    const int chunks = (K + 511) / 512;
+    // chunk number of this warp, and its step, as (row, chunk of the row)
+    const int64_t first = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5), step = int64_t(gridDim.x) * 8;
+    int64_t row = first / chunks;
+    int chunk = int(first - row * chunks);
+    const int64_t row_step = step / chunks;
+    const int chunk_step = int(step - row_step * chunks);
+    auto advance = [&]() {
+        row += row_step, chunk += chunk_step;
+        if (chunk >= chunks) chunk -= chunks, row++;
+    };
+    // two chunks at a time: the second one's load is in flight while the first is reduced
+    while (row < rows) {
+        uint32_t a[8 * sizeof(T) / 2], b[8 * sizeof(T) / 2];
+        const int64_t row_a = row;
+        const int chunk_a = chunk;
+        load_chunk<T, VEC>(x + row * K + chunk * 512 + lane * 16, K - chunk * 512 - lane * 16, a);
+        advance();
+        const int64_t row_b = row;
+        const int chunk_b = chunk;
+        load_chunk<T, VEC>(x + row * K + chunk * 512 + lane * 16, row < rows ? K - chunk * 512 - lane * 16 : 0, b);
+        advance();
+        quantize_chunk<T>(a, row_a, chunk_a, K, chunks, codes, ld, scale, sf);
+        if (row_b < rows) quantize_chunk<T>(b, row_b, chunk_b, K, chunks, codes, ld, scale, sf);
     }
 }
 
 // ---- tiles of 128 x 128 ---------------------------------------------------------------------
-// One CTA holds a tile in registers: lane l of warp w has columns 8 (l % 16) .. + 7 of rows
-// 16 w + l / 16 + 2 i.  kRows: blocks along the rows; kCols: blocks down the columns (kRows | kCols
-// from one read); kWeight: one block for the whole tile, its scale to both scale layouts.
+// kRows: blocks along the rows; kCols: blocks down the columns (kRows | kCols from one read);
+// kWeight: one block for the whole tile, its scale to both scale layouts.
+//
+// Persistent CTAs of 512 threads, two per SM; a thread owns 8 columns of 4 rows of a tile: lane l of
+// warp w has columns 8 (l % 16) .. + 7 of rows 8 w + l / 16 + 2 i.  bf16: each thread copies its own
+// 16-byte pieces of the next tiles to shared memory ahead of time (cp.async, waited for by itself:
+// the ring needs no barrier), so loads stay in flight while a tile is reduced; holding tiles in
+// registers without the ring left one CTA of 256 threads per SM and took 205 us for 16384 x 4096
+// in both forms.  fp32 tiles are loaded straight to registers (a ring of them leaves room for one CTA
+// per SM: 99 us against 61 for 8192 x 8192 weights).
+// bf16 magnitudes are compared two at a time as 16-bit integers.  Non-finite values (rare) are set
+// to zero for the maxima and patched into the codes afterwards.
 enum { kRows = 1, kCols = 2, kWeight = 4 };
 
 struct TileArgs {
@@ -124,17 +205,22 @@ struct TileArgs {
     const int *offsets;             // ragged row groups, or NULL
     int groups;
     int slots;                      // row tiles of one matrix (rows / 128 + groups with offsets)
+    int matrices;                   // kWeight
     uint8_t *codes;                 // row-wise (or weight) codes, pitch ld, in the input's row order
     int64_t ld;
-    float *scale;                   // kWeight: [matrix, row block, column block], or NULL
+    float *scale;                   // kRows: [row, column block]; kWeight: [matrix, row block, column block]; or NULL
     uint8_t *sf;                    // rows = slot rows, blocks along the columns
     uint8_t *codes_t;               // column-wise codes, pitch ld; groups: rows in slot order, zeros after a group's last
     uint8_t *sf_t;                  // rows = columns of x, blocks = row slots
 };
 
-// Slot t -> its group, first row and row count (0: no such tile).  Called by a whole warp.
+// Slot t -> its first row and row count (0: no such tile).  Called by a whole warp.
 __device__ __forceinline__ void slot_rows(const TileArgs &p, int t, int lane, int &row0, int &n)
 {
+    if (!p.offsets) {
+        row0 = 128 * t, n = min(128, p.rows - row0);
+        return;
+    }
     int below = 0;                                          // groups whose first slot is at or before t
     for (int g0 = 0; g0 < p.groups; g0 += 32) {
         const int g = g0 + lane;
@@ -148,132 +234,232 @@ __device__ __forceinline__ void slot_rows(const TileArgs &p, int t, int lane, in
     n = i < 0 ? 0 : max(0, min(128, hi - row0));
 }
 
+// A thread's 4 x 8 values: bf16 as 4 words per row, fp32 as 8.
+template <typename T> struct Piece {
+    using W = Word<T>;
+    static constexpr int WORDS = sizeof(T) == 2 ? 4 : 8, CHUNKS = WORDS / 4;
+    static constexpr int R = 4, THREADS = 2048 / R;
+    uint32_t u[R][WORDS];
+    // sets non-finite values to zero; bit 8 i + j: value (i, j) was one
+    __device__ __forceinline__ uint32_t drop_special()
+    {
+        uint32_t flags = 0;
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+            for (int w = 0; w < WORDS; w++) flags |= W::drop_special(u[i][w]) << (8 * i + 8 / WORDS * w);
+        return flags;
+    }
+    // fp32 bits of the largest magnitude of row i
+    __device__ __forceinline__ uint32_t row_max(int i) const
+    {
+        uint32_t m = u[i][0] & W::MAG;
+#pragma unroll
+        for (int w = 1; w < WORDS; w++) m = W::max_of(m, u[i][w] & W::MAG);
+        return W::fold(m);
+    }
+    // largest magnitudes of the R rows in word w: one (fp32) or two (bf16) columns
+    __device__ __forceinline__ uint32_t col_max(int w) const
+    {
+        uint32_t m = u[0][w] & W::MAG;
+#pragma unroll
+        for (int i = 1; i < R; i++) m = W::max_of(m, u[i][w] & W::MAG);
+        return m;
+    }
+};
+
+constexpr int kRing = 3;                                    // tiles of the ring: 96 KB, two CTAs per SM
+constexpr int kRingBytes = kRing * 128 * 128 * 2;
+
 template <typename T, bool VEC, int MODE>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(Piece<T>::THREADS, 2)
 fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    __shared__ uint32_t colmax[8][128];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    using P = Piece<T>;
+    using W = Word<T>;
+    constexpr int D = kRing, CH = P::CHUNKS, R = P::R, WARPS = P::THREADS / 32;
+    constexpr bool RING = VEC && sizeof(T) == 2;
+    extern __shared__ uint4 ring[];                        // [D][R rows][CH][thread]
+    __shared__ uint32_t colpart[WARPS][16 * P::WORDS];        // per warp: the columns' maxima (or, kWeight, one maximum)
+    __shared__ uint32_t colinv[16 * P::WORDS];              // reciprocal scales of the columns, as words
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kb = (p.cols + 127) / 128, kt = (kb + 3) / 4;
-    const int t = int(blockIdx.x / unsigned(kb)), cb = int(blockIdx.x - unsigned(t) * unsigned(kb));    // row slot, column block
-    int row0 = 128 * t, n = min(128, p.rows - row0);
-    if (!(MODE & kWeight) && p.offsets) slot_rows(p, t, lane, row0, n);
-    if (n <= 0) return;                                     // uniform over the CTA
-    const int64_t matrix = blockIdx.y;                      // 0 unless kWeight
-    const T *xm = x + matrix * p.rows * p.cols;
-    const int col = cb * 128 + 8 * (lane & 15), r0 = 16 * warp + (lane >> 4);
+    const int total = kb * p.slots * (MODE & kWeight ? p.matrices : 1);
+    const int r0 = 2 * R * warp + (lane >> 4), c0 = 8 * (lane & 15);
 
-    float v[8][8];
-    uint32_t amax_all = 0;
+    // Tiles are walked with the grid's stride; a cursor keeps a tile's row slot and column block.
+    struct Cursor { int tile, rest, cb; };                  // rest: row slot (kWeight: of all matrices)
+    const int rest_step = int(gridDim.x) / kb, cb_step = int(gridDim.x) - rest_step * kb;
+    auto advance = [&](Cursor &c) {
+        c.tile += gridDim.x, c.rest += rest_step, c.cb += cb_step;
+        if (c.cb >= kb) c.cb -= kb, c.rest++;
+    };
+    auto place = [&](const Cursor &c, int &t, int64_t &matrix, int &row0, int &n) {
+        matrix = MODE & kWeight ? c.rest / p.slots : 0;
+        t = MODE & kWeight ? c.rest - int(matrix) * p.slots : c.rest;
+        slot_rows(p, t, lane, row0, n);
+    };
+    auto fetch = [&](const Cursor &c, int stage) {          // one commit group per call, empty past the last tile
+        if (RING && c.tile < total) {
+            int t, row0, n;
+            int64_t matrix;
+            place(c, t, matrix, row0, n);
+            const int col = c.cb * 128 + c0;
+            const T *src = x + (matrix * p.rows + row0 + r0) * p.cols + col;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int r = r0 + 2 * i;
-        load_values<8, VEC>(xm + int64_t(row0 + r) * p.cols + col, r < n ? p.cols - col : 0, v[i]);
+            for (int i = 0; i < R; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) amax_all = max(amax_all, __float_as_uint(v[i][j]) & kAbs);
-    }
-    const bool special = __any_sync(0xFFFFFFFFu, amax_all >= kBitsInf);
-    // From here on non-finite values are NaN, and `mag` counts them as 0.
-    auto mag = [&](float f) { return special ? finite_abs(f) : __float_as_uint(f) & kAbs; };
-    if (special) {
-        amax_all = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[i][j] = finite_or_nan(v[i][j]), amax_all = max(amax_all, finite_abs(v[i][j]));
-    }
-
-    if constexpr (MODE & kWeight) {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) amax_all = max(amax_all, __shfl_xor_sync(0xFFFFFFFFu, amax_all, o));
-        if (lane == 0) colmax[0][warp] = amax_all;
-        __syncthreads();
-        uint32_t m = 0;
-#pragma unroll
-        for (int w = 0; w < 8; w++) m = max(m, colmax[0][w]);
-        const uint32_t e8 = fp8_e8m0(m);
-        const float inv = fp8_inv_scale(e8);
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int r = r0 + 2 * i;
-            if (r < n && col < p.cols)
-                *reinterpret_cast<uint2 *>(p.codes + (matrix * p.rows + row0 + r) * p.ld + col) =
-                    make_uint2(cvt_e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
-                               cvt_e4m3x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
-        }
-        const int nb = (p.rows + 127) / 128, nt = (nb + 3) / 4;
-        if (threadIdx.x == 0 && p.scale) p.scale[(matrix * nb + t) * kb + cb] = __uint_as_float(e8 << 23);
-        if (threadIdx.x < 128) {
-            if (p.sf) p.sf[matrix * nb * kt * 512 + sf_offset(uint32_t(128 * t + threadIdx.x), uint32_t(cb), uint32_t(kt))] = uint8_t(e8);
-            if (p.sf_t) p.sf_t[matrix * kb * nt * 512 + sf_offset(uint32_t(128 * cb + threadIdx.x), uint32_t(t), uint32_t(nt))] = uint8_t(e8);
-        }
-        return;
-    }
-
-    if constexpr (MODE & kRows) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int r = r0 + 2 * i;
-            uint32_t m = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) m = max(m, mag(v[i][j]));
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-            const uint32_t e8 = fp8_e8m0(m);
-            const float inv = fp8_inv_scale(e8);
-            if (r < n) {
-                if (col < p.cols)
-                    *reinterpret_cast<uint2 *>(p.codes + int64_t(row0 + r) * p.ld + col) =
-                        make_uint2(cvt_e4m3x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
-                                   cvt_e4m3x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
-                if ((lane & 15) == 0) {
-                    if (p.sf) p.sf[sf_offset(uint32_t(128 * t + r), uint32_t(cb), uint32_t(kt))] = uint8_t(e8);
-                    if (p.scale) p.scale[int64_t(row0 + r) * kb + cb] = __uint_as_float(e8 << 23);
+                for (int h = 0; h < CH; h++) {
+                    const bool in = r0 + 2 * i < n && col + 8 / CH * h < p.cols;
+                    const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(&ring[((stage * R + i) * CH + h) * P::THREADS + tid]));
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                 ::"r"(dst), "l"(in ? src + int64_t(2 * i) * p.cols + 8 / CH * h : x), "r"(in ? 16 : 0) : "memory");
                 }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+
+    Cursor now{int(blockIdx.x), int(blockIdx.x) / kb, int(blockIdx.x) % kb}, ahead = now;
+#pragma unroll
+    for (int d = 0; d < D; d++) {
+        fetch(ahead, d);
+        advance(ahead);
+    }
+    int stage = 0;
+    for (; now.tile < total; advance(now)) {
+        const int cb = now.cb;
+        int t, row0, n;
+        int64_t matrix;
+        place(now, t, matrix, row0, n);
+        asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
+        P v;
+        const int col = cb * 128 + c0;
+        if constexpr (VEC) {
+            const T *src = x + (matrix * p.rows + row0) * p.cols + col;
+#pragma unroll
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int h = 0; h < CH; h++) {
+                    uint4 q = make_uint4(0, 0, 0, 0);
+                    if (RING) q = ring[((stage * R + i) * CH + h) * P::THREADS + tid];
+                    else if (r0 + 2 * i < n && col + 8 / CH * h < p.cols)
+                        q = ld_stream(reinterpret_cast<const uint4 *>(src + int64_t(r0 + 2 * i) * p.cols + 8 / CH * h));
+                    v.u[i][4 * h] = q.x, v.u[i][4 * h + 1] = q.y, v.u[i][4 * h + 2] = q.z, v.u[i][4 * h + 3] = q.w;
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                load_ragged<P::WORDS>(x + (matrix * p.rows + row0 + r0 + 2 * i) * p.cols + col, r0 + 2 * i < n ? p.cols - col : 0, v.u[i]);
+        }
+        uint32_t m[R], most = 0;
+#pragma unroll
+        for (int i = 0; i < R; i++) m[i] = v.row_max(i), most = max(most, m[i]);
+        // every value has been used, so the loads above are done: refill their place in the ring
+        if (RING) {
+            fetch(ahead, stage);
+            advance(ahead);
+        }
+        stage = stage + 1 == D ? 0 : stage + 1;
+        if (n <= 0) continue;                               // a slot without rows; uniform over the CTA
+        uint32_t flags = 0;
+        const bool special = __any_sync(0xFFFFFFFFu, most >= kBitsInf);
+        if (special) {
+            flags = v.drop_special();
+            most = 0;
+#pragma unroll
+            for (int i = 0; i < R; i++) m[i] = v.row_max(i), most = max(most, m[i]);
+        }
+        auto put = [&](uint8_t *dst, int i, const uint32_t (&inv)[P::WORDS]) {
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(W::codes(v.u[i], inv), W::codes(v.u[i] + P::WORDS / 2, inv + P::WORDS / 2));
+            if (special) store_nans(dst, (flags >> (8 * i)) & 0xFFu);
+        };
+        auto put_all = [&](uint8_t *dst, int i, uint32_t s) {      // one scale for the row's values
+            uint32_t inv[P::WORDS];
+#pragma unroll
+            for (int w = 0; w < P::WORDS; w++) inv[w] = s;
+            put(dst, i, inv);
+        };
+
+        if constexpr (MODE & kWeight) {
+            uint32_t a = __reduce_max_sync(0xFFFFFFFFu, most);
+            if (lane == 0) colpart[warp][0] = a;
+            __syncthreads();
+            a = __reduce_max_sync(0xFFFFFFFFu, colpart[lane % WARPS][0]);
+            const uint32_t e8 = fp8_e8m0(a);
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                if (r0 + 2 * i < n && col < p.cols) put_all(p.codes + (matrix * p.rows + row0 + r0 + 2 * i) * p.ld + col, i, W::inv(e8));
+            const int nb = p.slots, nt = (nb + 3) / 4;
+            if (tid == 0 && p.scale) p.scale[(matrix * nb + t) * kb + cb] = __uint_as_float(e8 << 23);
+            if (tid < 128) {
+                if (p.sf) p.sf[matrix * nb * kt * 512 + sf_offset(uint32_t(128 * t + tid), uint32_t(cb), uint32_t(kt))] = uint8_t(e8);
+                if (p.sf_t) p.sf_t[matrix * kb * nt * 512 + sf_offset(uint32_t(128 * cb + tid), uint32_t(t), uint32_t(nt))] = uint8_t(e8);
+            }
+            __syncthreads();                                // colpart is written again for the next tile
+            continue;
+        }
+
+        if constexpr (MODE & kCols) {
+#pragma unroll
+            for (int w = 0; w < P::WORDS; w++) {
+                uint32_t a = v.col_max(w);
+                a = W::max_of(a, __shfl_xor_sync(0xFFFFFFFFu, a, 16));
+                if (lane < 16) colpart[warp][P::WORDS * lane + w] = a;
             }
         }
-    }
-    if constexpr (MODE & kCols) {
-        uint32_t m[8];
+        if constexpr (MODE & kRows) {
+            // Maxima of the 4 rows over 16 lanes: two exchanges that halve what a lane keeps (its row is
+            // then the upper two of its four lane bits), two plain steps, and the scales sent back:
+            // 9 shuffles instead of 16.
+            const bool b3 = lane & 8, b2 = lane & 4;
+            const uint32_t x0 = __shfl_xor_sync(0xFFFFFFFFu, b3 ? m[0] : m[2], 8), x1 = __shfl_xor_sync(0xFFFFFFFFu, b3 ? m[1] : m[3], 8);
+            const uint32_t y0 = max(b3 ? m[2] : m[0], x0), y1 = max(b3 ? m[3] : m[1], x1);
+            uint32_t z = max(b2 ? y1 : y0, __shfl_xor_sync(0xFFFFFFFFu, b2 ? y0 : y1, 4));
+            z = max(z, __shfl_xor_sync(0xFFFFFFFFu, z, 2));
+            z = max(z, __shfl_xor_sync(0xFFFFFFFFu, z, 1));
+            const uint32_t e8 = fp8_e8m0(z);
+            constexpr int SHARE = 16 / R;                   // lanes that end up with the same row
+            const int mine = r0 + 2 * ((lane & 15) / SHARE);
+            if (lane % SHARE == 0 && mine < n) {
+                if (p.sf) p.sf[sf_offset(uint32_t(128 * t + mine), uint32_t(cb), uint32_t(kt))] = uint8_t(e8);
+                if (p.scale) p.scale[int64_t(row0 + mine) * kb + cb] = __uint_as_float(e8 << 23);
+            }
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            m[j] = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i++) m[j] = max(m[j], mag(v[i][j]));
-            m[j] = max(m[j], __shfl_xor_sync(0xFFFFFFFFu, m[j], 16));
+            for (int i = 0; i < R; i++) {
+                const uint32_t s = W::inv(__shfl_sync(0xFFFFFFFFu, e8, (lane & 16) | (i * SHARE)));
+                if (r0 + 2 * i < n && col < p.cols) put_all(p.codes + int64_t(row0 + r0 + 2 * i) * p.ld + col, i, s);
+            }
         }
-        if (lane < 16) {
+        if constexpr (MODE & kCols) {
+            __syncthreads();
+            if (tid < 16 * P::WORDS) {                      // one word of columns per thread
+                uint32_t a = 0;
 #pragma unroll
-            for (int j = 0; j < 8; j++) colmax[warp][8 * lane + j] = m[j];
-        }
-        __syncthreads();
-        float inv[8];
-        uint32_t e8[8];
+                for (int w = 0; w < WARPS; w++) a = W::max_of(a, colpart[w][tid]);
+                const int st = (p.slots + 3) / 4;
+                if constexpr (sizeof(T) == 2) {
+                    const uint32_t e0 = fp8_e8m0(a << 16), e1 = fp8_e8m0(a & 0xFFFF0000u);
+                    colinv[tid] = (W::inv(e0) & 0xFFFFu) | (W::inv(e1) & 0xFFFF0000u);
+                    p.sf_t[sf_offset(uint32_t(cb * 128 + 2 * tid), uint32_t(t), uint32_t(st))] = uint8_t(e0);
+                    p.sf_t[sf_offset(uint32_t(cb * 128 + 2 * tid + 1), uint32_t(t), uint32_t(st))] = uint8_t(e1);
+                } else {
+                    const uint32_t e0 = fp8_e8m0(a);
+                    colinv[tid] = W::inv(e0);
+                    p.sf_t[sf_offset(uint32_t(cb * 128 + tid), uint32_t(t), uint32_t(st))] = uint8_t(e0);
+                }
+            }
+            __syncthreads();
+            uint32_t inv[P::WORDS];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            uint32_t a = 0;
+            for (int w = 0; w < P::WORDS; w++) inv[w] = colinv[P::WORDS * (lane & 15) + w];
+            // Groups: the tile goes to its slot's rows, all 128 of them, so that the product over a
+            // group's rows runs in whole blocks (the values past the group are zeros).
+            const int64_t out0 = p.offsets ? 128ll * t : row0;
+            const int out_n = p.offsets ? 128 : n;
 #pragma unroll
-            for (int w = 0; w < 8; w++) a = max(a, colmax[w][8 * (lane & 15) + j]);
-            e8[j] = fp8_e8m0(a);
-            inv[j] = fp8_inv_scale(e8[j]);
-        }
-        // Groups: the tile goes to its slot's rows, all 128 of them, so that the product over a
-        // group's rows runs in whole blocks (the values past the group are zeros).
-        const int64_t out0 = p.offsets ? 128ll * t : row0;
-        const int out_n = p.offsets ? 128 : n;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int r = r0 + 2 * i;
-            if (r < out_n && col < p.cols)
-                *reinterpret_cast<uint2 *>(p.codes_t + (out0 + r) * p.ld + col) =
-                    make_uint2(cvt_e4m3x4(v[i][0] * inv[0], v[i][1] * inv[1], v[i][2] * inv[2], v[i][3] * inv[3]),
-                               cvt_e4m3x4(v[i][4] * inv[4], v[i][5] * inv[5], v[i][6] * inv[6], v[i][7] * inv[7]));
-        }
-        if (warp == 0 && lane < 16) {
-            const int st = (p.slots + 3) / 4;
-#pragma unroll
-            for (int j = 0; j < 8; j++) p.sf_t[sf_offset(uint32_t(col + j), uint32_t(t), uint32_t(st))] = uint8_t(e8[j]);
+            for (int i = 0; i < R; i++)
+                if (r0 + 2 * i < out_n && col < p.cols) put(p.codes_t + (out0 + r0 + 2 * i) * p.ld + col, i, inv);
         }
     }
 }
@@ -311,28 +497,42 @@ int check_groups(const int *offsets, int64_t groups)
     return LS_OK;
 }
 
-// 16-byte loads of whole runs of `run` values
+// rows made of whole runs of `run` values, each on a boundary of its size
 bool vectorizes(const void *x, int dtype, int64_t K, int run)
 {
-    return aligned16(x) && K % run == 0 && (K * (dtype == LS_BF16 ? 2 : 4)) % 16 == 0;
+    const uintptr_t bytes = std::min<uintptr_t>(32, uintptr_t(run) * (dtype == LS_BF16 ? 2 : 4));
+    return reinterpret_cast<uintptr_t>(x) % bytes == 0 && K % run == 0;
+}
+
+template <typename T, bool VEC, int MODE>
+int launch_tile_kernel(const void *x, const TileArgs &p, int64_t tiles, cudaStream_t st)
+{
+    constexpr int ring = VEC && sizeof(T) == 2 ? kRingBytes : 0;
+    static bool attr_set[64] = {};
+    int dev = 0;
+    if (int rc = current_device(&dev)) return rc;
+    {
+        std::lock_guard<std::mutex> lk(state_mutex());
+        if (!attr_set[dev]) {
+            LS_CUDA(cudaFuncSetAttribute(fp8_tile_kernel<T, VEC, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, ring));
+            attr_set[dev] = true;
+        }
+    }
+    const int64_t most = int64_t(sm_count()) * 2;
+    fp8_tile_kernel<T, VEC, MODE><<<unsigned(std::min(tiles, most)), Piece<T>::THREADS, ring, st>>>(static_cast<const T *>(x), p);
+    LS_LAUNCH_CHECK("fp8_tile_kernel");
+    return LS_OK;
 }
 
 template <int MODE>
-int launch_tiles(const void *x, int dtype, const TileArgs &p, int64_t matrices, cudaStream_t st)
+int launch_tiles(const void *x, int dtype, const TileArgs &p, cudaStream_t st)
 {
-    const int64_t tiles = int64_t((p.cols + 127) / 128) * p.slots;
-    if (tiles > 0x7FFFFFFFll) return fail(LS_EINVAL, "too many tiles of 128 x 128");
-    const dim3 grid{unsigned(tiles), unsigned(matrices), 1};
-    const bool vec = vectorizes(x, dtype, p.cols, 8);
-    if (dtype == LS_BF16) {
-        if (vec) fp8_tile_kernel<__nv_bfloat16, true, MODE><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16 *>(x), p);
-        else fp8_tile_kernel<__nv_bfloat16, false, MODE><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16 *>(x), p);
-    } else {
-        if (vec) fp8_tile_kernel<float, true, MODE><<<grid, 256, 0, st>>>(static_cast<const float *>(x), p);
-        else fp8_tile_kernel<float, false, MODE><<<grid, 256, 0, st>>>(static_cast<const float *>(x), p);
-    }
-    LS_LAUNCH_CHECK("fp8_tile_kernel");
-    return LS_OK;
+    const int64_t tiles = int64_t((p.cols + 127) / 128) * p.slots * p.matrices;
+    if (tiles > 0x3FFFFFFFll) return fail(LS_EINVAL, "too many tiles of 128 x 128");
+    const bool vec = vectorizes(x, dtype, p.cols, dtype == LS_BF16 ? 8 : 4);
+    if (dtype == LS_BF16)
+        return vec ? launch_tile_kernel<__nv_bfloat16, true, MODE>(x, p, tiles, st) : launch_tile_kernel<__nv_bfloat16, false, MODE>(x, p, tiles, st);
+    return vec ? launch_tile_kernel<float, true, MODE>(x, p, tiles, st) : launch_tile_kernel<float, false, MODE>(x, p, tiles, st);
 }
 
 }  // namespace
@@ -353,10 +553,10 @@ extern "C" int ls_quantize_fp8(const void *x, int dtype, int64_t rows, int64_t K
     if (!aligned16(codes) || !aligned16(sf) || !aligned16(scale)) return fail(LS_EALIGN, "codes and scales must be 16-byte aligned");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (offsets) {
-        TileArgs p{int(rows), int(K), offsets, int(groups), int(fp8_slots(rows, groups)), codes, ld, scale, sf, nullptr, nullptr};
-        return launch_tiles<kRows>(x, dtype, p, 1, st);
+        TileArgs p{int(rows), int(K), offsets, int(groups), int(fp8_slots(rows, groups)), 1, codes, ld, scale, sf, nullptr, nullptr};
+        return launch_tiles<kRows>(x, dtype, p, st);
     }
-    const int64_t warps = rows * ((K + 511) / 512), want = (warps + 7) / 8, most = int64_t(sm_count()) * 16;
+    const int64_t warps = rows * ((K + 511) / 512), want = (warps + 7) / 8, most = int64_t(sm_count()) * 4;
     const unsigned grid = unsigned(want < most ? want : most);
     const bool vec = vectorizes(x, dtype, K, 16);
     if (dtype == LS_BF16) {
@@ -382,10 +582,10 @@ extern "C" int ls_quantize_fp8_both(const void *x, int dtype, int64_t rows, int6
     if (!aligned16(codes) || !aligned16(sf) || !aligned16(codes_t) || !aligned16(sf_t))
         return fail(LS_EALIGN, "codes and scales must be 16-byte aligned");
     const int64_t slots = offsets ? fp8_slots(rows, groups) : (rows + 127) / 128;
-    TileArgs p{int(rows), int(K), offsets, int(groups), int(slots), codes, ld, nullptr, sf, codes_t, sf_t};
+    TileArgs p{int(rows), int(K), offsets, int(groups), int(slots), 1, codes, ld, nullptr, sf, codes_t, sf_t};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!codes) return launch_tiles<kCols>(x, dtype, p, 1, st);
-    return launch_tiles<kRows | kCols>(x, dtype, p, 1, st);
+    if (!codes) return launch_tiles<kCols>(x, dtype, p, st);
+    return launch_tiles<kRows | kCols>(x, dtype, p, st);
 }
 
 extern "C" int ls_quantize_fp8_weight(const void *w, int dtype, int64_t matrices, int64_t N, int64_t K, uint8_t *codes,
@@ -397,8 +597,8 @@ extern "C" int ls_quantize_fp8_weight(const void *w, int dtype, int64_t matrices
     if (!codes) return fail(LS_EINVAL, "null pointer");
     if (!aligned16(codes) || !aligned16(sf) || !aligned16(sf_t) || !aligned16(scale))
         return fail(LS_EALIGN, "codes and scales must be 16-byte aligned");
-    TileArgs p{int(N), int(K), nullptr, 0, int((N + 127) / 128), codes, ld, scale, sf, nullptr, sf_t};
-    return launch_tiles<kWeight>(w, dtype, p, matrices, static_cast<cudaStream_t>(stream));
+    TileArgs p{int(N), int(K), nullptr, 0, int((N + 127) / 128), int(matrices), codes, ld, scale, sf, nullptr, sf_t};
+    return launch_tiles<kWeight>(w, dtype, p, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int ls_dequantize_fp8(const uint8_t *codes, int64_t ld, const float *scale, int64_t rows, int64_t K,

@@ -21,7 +21,7 @@ grouped products with the same offsets.
 import torch
 
 from . import _lib
-from ._lib import aligned, check, lib, on_device_of, ptr, stream
+from ._lib import check, lib, on_device_of
 
 FP8_MAX = 448.0
 BLOCK = 128
@@ -29,74 +29,107 @@ MAX_GROUPS = 1024
 _CODES = torch.float8_e4m3fn
 
 
+# Serving calls take microseconds, and so do the host's own steps: pointers go to ctypes as plain
+# integers, and sizes are computed here.
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream if _raw_stream is None else _raw_stream(t.get_device())
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_DTYPE = {torch.float32: _lib.LS_F32, torch.bfloat16: _lib.LS_BF16}
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _aligned(t):
+    return t if t.is_contiguous() and t.data_ptr() % 32 == 0 else _lib.aligned(t, 32)
+
+
+def _out_code(dtype):
+    code = _DTYPE.get(dtype)
+    return _lib.dtype_code(dtype) if code is None else code       # raises for the others
+
+
 def sf_bytes(rows: int, K: int) -> int:
     """Size of the scale-factor buffer of a [rows, K] operand with blocks along K."""
-    return int(lib().ls_fp8_sf_bytes(rows, K))
+    return ((rows + 127) // 128) * ((K + 511) // 512) * 512
 
 
 def slots(rows: int, groups: int) -> int:
     """Row tiles of 128 that a tensor of `rows` rows in `groups` ragged groups may take (see ls_fp8_slots)."""
-    return int(lib().ls_fp8_slots(rows, groups))
+    return rows // 128 + groups
 
 
 def _input(x, dims=2):
     if x.dim() != dims:
         raise ValueError(f"expected a {dims}-dimensional tensor, got shape {tuple(x.shape)}")
-    if x.dtype not in (torch.float32, torch.bfloat16):
+    if x.dtype not in _DTYPE:
         x = x.float()
-    return aligned(x)
+    return _aligned(x)
+
+
+def _pitch(K):
+    return (K + 15) // 16 * 16
 
 
 def _codes(lead, rows, K, device):
-    pitch = -(-K // 16) * 16
-    return torch.empty((*lead, rows, pitch), dtype=_CODES, device=device)[..., :K]
+    if K % 16 == 0:
+        return torch.empty((*lead, rows, K), dtype=_CODES, device=device)
+    return torch.empty((*lead, rows, _pitch(K)), dtype=_CODES, device=device)[..., :K]
+
+
+def _bytes(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _pitched(codes):
     """(codes, row pitch) as the products read them: rows 16-byte aligned, matrices back to back."""
-    if codes.dtype == torch.uint8:
-        codes = codes.view(_CODES)
     if codes.dtype != _CODES:
-        raise TypeError(f"codes must be float8_e4m3fn (or their bytes), got {codes.dtype}")
-    *lead, rows, K = codes.shape
-    ld = codes.stride(-2) if rows > 1 else max(codes.stride(-2), -(-K // 16) * 16)
-    if rows == 1 and ld % 16:
-        ld = -(-K // 16) * 16
-    ok = (K <= 1 or codes.stride(-1) == 1) and ld >= K and ld % 16 == 0 and codes.data_ptr() % 16 == 0
-    if lead and lead[0] > 1:
-        ok = ok and codes.stride(0) == rows * ld
-    if not ok:
-        fresh = _codes(lead, rows, K, codes.device)
-        fresh.view(torch.uint8).copy_(codes.view(torch.uint8)) if codes.stride(-1) == 1 or K <= 1 else \
-            fresh.view(torch.uint8).copy_(codes.contiguous().view(torch.uint8))
-        codes, ld = fresh, fresh.stride(-2) if rows > 1 else -(-K // 16) * 16
-    return codes, ld
+        if codes.dtype != torch.uint8:
+            raise TypeError(f"codes must be float8_e4m3fn (or their bytes), got {codes.dtype}")
+        codes = codes.view(_CODES)
+    rows, K = codes.shape[-2:]
+    ld = codes.stride(-2)
+    if rows == 1 and (ld < K or ld % 16):                     # the pitch of a single row is free
+        ld = _pitch(K) if codes.dim() == 2 else 0
+    if (codes.stride(-1) == 1 or K <= 1) and ld >= K and ld % 16 == 0 and codes.data_ptr() % 16 == 0 and \
+            (codes.dim() == 2 or codes.shape[0] <= 1 or codes.stride(0) == rows * ld):
+        return codes, ld
+    fresh = _codes(codes.shape[:-2], rows, K, codes.device)
+    fresh.view(torch.uint8).copy_(codes.view(torch.uint8))
+    return fresh, _pitch(K)
 
 
-def _groups(offsets, device):
+def _groups(offsets):
     """(int32 offsets, number of groups)."""
-    if offsets.dim() != 1 or offsets.numel() < 2 or offsets.numel() > MAX_GROUPS + 1:
+    if offsets is None:
+        return None, 0
+    if offsets.dim() != 1 or not 2 <= offsets.shape[0] <= MAX_GROUPS + 1:
         raise ValueError(f"offsets: groups + 1 values, 1 to {MAX_GROUPS} groups; got shape {tuple(offsets.shape)}")
-    if offsets.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"offsets must be int32 or int64, got {offsets.dtype}")
-    return offsets.to(torch.int32).contiguous(), offsets.numel() - 1
+    if offsets.dtype != torch.int32:
+        if offsets.dtype != torch.int64:
+            raise TypeError(f"offsets must be int32 or int64, got {offsets.dtype}")
+        offsets = offsets.to(torch.int32)
+    return offsets.contiguous(), offsets.shape[0] - 1
 
 
 def _quantize_rows(x, offsets, want_scale, want_sf):
     with on_device_of(x, offsets):
-        *lead, K = x.shape
-        x = _input(x.reshape(-1, K) if x.dim() != 2 else x)
-        rows = x.shape[0]
-        off, G = (None, 0) if offsets is None else _groups(offsets, x.device)
-        codes = _codes((), rows, K, x.device)
-        scale = torch.empty((rows, -(-K // BLOCK)), dtype=torch.float32, device=x.device) if want_scale else None
-        sf_rows = rows if off is None else BLOCK * slots(rows, G)
-        sf = torch.empty(sf_bytes(sf_rows, K), dtype=torch.uint8, device=x.device) if want_sf else None
-        check(lib().ls_quantize_fp8(ptr(x), _lib.dtype_code(x.dtype), rows, K, ptr(off), G, ptr(codes), -(-K // 16) * 16,
-                                    ptr(scale), ptr(sf), stream()))
-        if len(lead) != 1:
-            codes = codes.view(*lead, K) if codes.is_contiguous() else codes.unflatten(0, lead)
-            scale = None if scale is None else scale.view(*lead, -1)
+        shape = x.shape
+        K = shape[-1]
+        x = _input(x if len(shape) == 2 else x.reshape(-1, K))
+        rows, dev = x.shape[0], x.device
+        off, G = _groups(offsets)
+        codes = _codes((), rows, K, dev)
+        scale = torch.empty((rows, -(-K // BLOCK)), dtype=torch.float32, device=dev) if want_scale else None
+        sf = _bytes(sf_bytes(rows if off is None else BLOCK * slots(rows, G), K), dev) if want_sf else None
+        check(lib().ls_quantize_fp8(x.data_ptr(), _DTYPE[x.dtype], rows, K, _ptr(off), G, codes.data_ptr(), _pitch(K),
+                                    _ptr(scale), _ptr(sf), _stream(x)))
+        if len(shape) != 2:
+            codes = codes.view(shape) if K % 16 == 0 else codes.unflatten(0, shape[:-1]) if len(shape) > 2 else codes[0]
+            scale = None if scale is None else scale.view(*shape[:-1], -1)
         return codes, scale, sf
 
 
@@ -123,14 +156,15 @@ def quantize_fp8_both(x: torch.Tensor, offsets: torch.Tensor = None, rows_too: b
     with on_device_of(x, offsets):
         x = _input(x)
         rows, K = x.shape
-        off, G = (None, 0) if offsets is None else _groups(offsets, x.device)
+        dev = x.device
+        off, G = _groups(offsets)
         sf_rows = rows if off is None else BLOCK * slots(rows, G)
-        codes = _codes((), rows, K, x.device) if rows_too else None
-        sf = torch.empty(sf_bytes(sf_rows, K), dtype=torch.uint8, device=x.device) if rows_too else None
-        codes_t = _codes((), sf_rows, K, x.device)
-        sf_t = torch.empty(sf_bytes(K, sf_rows), dtype=torch.uint8, device=x.device)
-        check(lib().ls_quantize_fp8_both(ptr(x), _lib.dtype_code(x.dtype), rows, K, ptr(off), G, ptr(codes), ptr(sf),
-                                         ptr(codes_t), ptr(sf_t), -(-K // 16) * 16, stream()))
+        codes = _codes((), rows, K, dev) if rows_too else None
+        sf = _bytes(sf_bytes(sf_rows, K), dev) if rows_too else None
+        codes_t = _codes((), sf_rows, K, dev)
+        sf_t = _bytes(sf_bytes(K, sf_rows), dev)
+        check(lib().ls_quantize_fp8_both(x.data_ptr(), _DTYPE[x.dtype], rows, K, _ptr(off), G, _ptr(codes), _ptr(sf),
+                                         codes_t.data_ptr(), sf_t.data_ptr(), _pitch(K), _stream(x)))
         return codes, sf, codes_t, sf_t
 
 
@@ -138,17 +172,16 @@ def quantize_fp8_weight(w: torch.Tensor, want_scale: bool = False):
     """w [N, K] or [groups, N, K] -> (codes, sf, sf_t[, scale fp32 [..., N / 128, K / 128]]) with one
     scale per 128 x 128; sf serves products over K, sf_t (the transpose's) products over N."""
     with on_device_of(w):
-        w = _input(w, w.dim() if w.dim() in (2, 3) else 2)
+        w = _input(w, 3 if w.dim() == 3 else 2)
         *lead, N, K = w.shape
-        G = lead[0] if lead else 1
+        G, dev = lead[0] if lead else 1, w.device
         if G > MAX_GROUPS:
             raise ValueError(f"at most {MAX_GROUPS} matrices, got {G}")
-        codes = _codes(lead, N, K, w.device)
-        sf = torch.empty((*lead, sf_bytes(N, K)), dtype=torch.uint8, device=w.device)
-        sf_t = torch.empty((*lead, sf_bytes(K, N)), dtype=torch.uint8, device=w.device)
-        scale = torch.empty((*lead, -(-N // BLOCK), -(-K // BLOCK)), dtype=torch.float32, device=w.device) if want_scale else None
-        check(lib().ls_quantize_fp8_weight(ptr(w), _lib.dtype_code(w.dtype), G, N, K, ptr(codes), -(-K // 16) * 16, ptr(scale),
-                                           ptr(sf), ptr(sf_t), stream()))
+        codes = _codes(lead, N, K, dev)
+        sf, sf_t = _bytes((*lead, sf_bytes(N, K)), dev), _bytes((*lead, sf_bytes(K, N)), dev)
+        scale = torch.empty((*lead, -(-N // BLOCK), -(-K // BLOCK)), dtype=torch.float32, device=dev) if want_scale else None
+        check(lib().ls_quantize_fp8_weight(w.data_ptr(), _DTYPE[w.dtype], G, N, K, codes.data_ptr(), _pitch(K), _ptr(scale),
+                                           sf.data_ptr(), sf_t.data_ptr(), _stream(w)))
         return (codes, sf, sf_t, scale) if want_scale else (codes, sf, sf_t)
 
 
@@ -162,14 +195,16 @@ def dequantize_fp8(codes: torch.Tensor, scale: torch.Tensor, out_dtype=torch.flo
         if row_block == BLOCK and scale.shape != (*lead, -(-rows // BLOCK), kb):
             raise ValueError(f"scale shape {tuple(scale.shape)} does not fit codes {tuple(codes.shape)}")
         out = torch.empty(codes.shape, dtype=out_dtype, device=codes.device)
-        scale = aligned(scale.float())
-        if row_block == 1:
-            codes, ld = _pitched(codes.reshape(-1, K))
-            check(lib().ls_dequantize_fp8(ptr(codes), ld, ptr(scale), codes.shape[0], K, 1, ptr(out), _lib.dtype_code(out_dtype), stream()))
-            return out
-        for c, s, o in zip(codes.reshape(-1, rows, K), scale.reshape(-1, -(-rows // BLOCK), kb), out.view(-1, rows, K)):
+        scale = _aligned(scale.float())
+
+        def one(c, s, o):
             c, ld = _pitched(c)
-            check(lib().ls_dequantize_fp8(ptr(c), ld, ptr(s), rows, K, BLOCK, ptr(o), _lib.dtype_code(out_dtype), stream()))
+            check(lib().ls_dequantize_fp8(c.data_ptr(), ld, s.data_ptr(), *c.shape, row_block, o.data_ptr(), _out_code(out_dtype), _stream(o)))
+        if row_block == 1:
+            one(codes.reshape(-1, K), scale, out)
+        else:
+            for c, s, o in zip(codes.reshape(-1, rows, K), scale.reshape(-1, -(-rows // BLOCK), kb), out.view(-1, rows, K)):
+                one(c, s, o)
         return out
 
 
@@ -194,18 +229,23 @@ def scales_to_sf(scale: torch.Tensor, rows: int = None):
 _NT, _NN, _TN = 0, 1, 2
 
 
-def _sf(sf, matrices, rows, K, what):
-    want = matrices * sf_bytes(rows, K)
+def _sf(sf, want, what):
     if sf.dtype != torch.uint8 or sf.numel() != want:
         raise ValueError(f"{what}: a scale-factor buffer of {want} bytes is needed, got {sf.numel()} of {sf.dtype}")
-    return aligned(sf)
+    return _aligned(sf)
+
+
+def _given(out, shape, dtype):
+    if out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 16:
+        raise ValueError(f"out must be a contiguous, 16-byte aligned {tuple(shape)} tensor of {dtype}")
+    return out
 
 
 def _product(form, a, b, a_sf, b_sf, out_dtype, out, offsets, rows):
     with on_device_of(a, b, a_sf, b_sf, offsets, out):
         if a.dim() != 2 or b.dim() != (2 if offsets is None or form == _TN else 3):
             raise ValueError(f"operand shapes {tuple(a.shape)} and {tuple(b.shape)}")
-        off, G = (None, 1) if offsets is None else _groups(offsets, a.device)
+        off, G = _groups(offsets) if offsets is not None else (None, 1)
         if form == _TN:
             held, M = a.shape
             N = b.shape[1]
@@ -214,28 +254,25 @@ def _product(form, a, b, a_sf, b_sf, out_dtype, out, offsets, rows):
             if b.shape[0] != held or (off is not None and held != tiles):
                 raise ValueError(f"operands with {a.shape[0]} and {b.shape[0]} rows"
                                  + ("" if off is None else f", {tiles} needed for {K} rows in {G} groups"))
-            a_sf, b_sf = _sf(a_sf, 1, M, tiles, "a_sf"), _sf(b_sf, 1, N, tiles, "b_sf")
+            a_sf, b_sf = _sf(a_sf, sf_bytes(M, tiles), "a_sf"), _sf(b_sf, sf_bytes(N, tiles), "b_sf")
             shape = (M, N) if off is None else (G, M, N)
         else:
             M, K = a.shape
             N, Kb = b.shape[-2:] if form == _NT else b.shape[-1:-3:-1]
             if Kb != K or (off is not None and b.shape[0] != G):
                 raise ValueError(f"operand shapes {tuple(a.shape)} and {tuple(b.shape)} do not fit" + ("" if off is None else f" {G} groups"))
-            a_sf = _sf(a_sf, 1, M if off is None else BLOCK * slots(M, G), K, "a_sf")
-            b_sf = _sf(b_sf, G, N, K, "b_sf")
+            a_sf = _sf(a_sf, sf_bytes(M if off is None else BLOCK * slots(M, G), K), "a_sf")
+            b_sf = _sf(b_sf, G * sf_bytes(N, K), "b_sf")
             shape = (M, N)
         (a, lda), (b, ldb) = _pitched(a), _pitched(b)
-        if out is None:
-            c = torch.empty(shape, dtype=out_dtype, device=a.device)
-        else:
-            if out.shape != shape or out.dtype != out_dtype or not out.is_contiguous() or out.data_ptr() % 16:
-                raise ValueError(f"out must be a contiguous, 16-byte aligned {tuple(shape)} tensor of {out_dtype}")
-            c = out
-        args = (form, ptr(a), lda, ptr(b), ldb, ptr(a_sf), ptr(b_sf), ptr(c), _lib.dtype_code(out_dtype), M, N, K)
+        code = _out_code(out_dtype)
+        c = torch.empty(shape, dtype=out_dtype, device=a.device) if out is None else _given(out, shape, out_dtype)
         if off is None:
-            check(lib().ls_fp8_gemm(*args, stream()))
+            check(lib().ls_fp8_gemm(form, a.data_ptr(), lda, b.data_ptr(), ldb, a_sf.data_ptr(), b_sf.data_ptr(), c.data_ptr(), code,
+                                    M, N, K, _stream(a)))
         else:
-            check(lib().ls_fp8_gemm_grouped(*args, ptr(off), G, 1 if out is None else 0, stream()))
+            check(lib().ls_fp8_gemm_grouped(form, a.data_ptr(), lda, b.data_ptr(), ldb, a_sf.data_ptr(), b_sf.data_ptr(), c.data_ptr(),
+                                            code, M, N, K, off.data_ptr(), G, 1 if out is None else 0, _stream(a)))
         return c
 
 

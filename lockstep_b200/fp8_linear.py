@@ -14,10 +14,16 @@ where each expert's rows start, and the weight is [experts, out, in].
 There is no CPU path.
 """
 
+import functools
+
 import torch
 import torch.nn as nn
 
-from . import fp8
+from . import _lib, fp8
+from ._lib import check, lib, on_device_of
+
+_SERVE, _FORWARD, _SAVED, _BACKWARD = range(4)
+_GRAD_X, _GRAD_W = 1, 2
 
 
 def _check(x, w, dims):
@@ -25,58 +31,67 @@ def _check(x, w, dims):
         raise ValueError(f"weight must be {dims}-dimensional, got shape {tuple(w.shape)}")
     if x.shape[-1] != w.shape[-1]:
         raise ValueError(f"input of width {x.shape[-1]} for a weight of shape {tuple(w.shape)}")
-    if x.dtype not in (torch.float32, torch.bfloat16):
+    if x.dtype not in fp8._DTYPE:
         raise TypeError(f"unsupported dtype {x.dtype}")
+
+
+@functools.lru_cache(maxsize=4096)
+def _buffer_bytes(what, rows, N, K, groups, grads):
+    return max(16, int(lib().ls_fp8_linear_bytes(what, rows, N, K, groups, grads)))
+
+
+def _buffer(what, rows, N, K, groups, grads, device):
+    return torch.empty(_buffer_bytes(what, rows, N, K, groups, grads), dtype=torch.uint8, device=device)
+
+
+def _rows_of(x, w, offsets):
+    """(int32 offsets or None, groups as the sizes count them, as the calls do) after checking them against w."""
+    off, G = fp8._groups(offsets)
+    if off is not None and w.shape[0] != G:
+        raise ValueError(f"{w.shape[0]} experts for offsets of {G} groups")
+    return off, G, max(G, 1)
 
 
 class _FP8Matmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
-        wc, wsf, wsf_t = fp8.quantize_fp8_weight(w)
-        if ctx.needs_input_grad[1]:
-            xc, xsf, xct, xsf_t = fp8.quantize_fp8_both(x, offsets)
-        else:
-            (xc, xsf), xct, xsf_t = fp8.quantize_fp8_packed(x, offsets), None, None
-        keep_w = ctx.needs_input_grad[0]
-        ctx.save_for_backward(offsets, xct, xsf_t, wc if keep_w else None, wsf_t if keep_w else None)
-        ctx.rows, ctx.dtypes = x.shape[0], (x.dtype, w.dtype)
-        if offsets is None:
-            return fp8.fp8_gemm(xc, wc, xsf, wsf, x.dtype)
-        return fp8.fp8_gemm_grouped(xc, wc, xsf, wsf, offsets, x.dtype)
+        with on_device_of(x, w, offsets):
+            off, G, calls = _rows_of(x, w, offsets)
+            xi, wi = fp8._aligned(x), fp8._input(w, w.dim())
+            (rows, K), N, dev = xi.shape, w.shape[-2], x.device
+            grads = (_GRAD_X if ctx.needs_input_grad[0] else 0) | (_GRAD_W if ctx.needs_input_grad[1] else 0)
+            y = torch.empty((rows, N), dtype=x.dtype, device=dev)
+            work = _buffer(_FORWARD, rows, N, K, G, grads, dev)
+            saved = _buffer(_SAVED, rows, N, K, G, grads, dev) if grads else None
+            check(lib().ls_fp8_linear_forward(xi.data_ptr(), fp8._DTYPE[xi.dtype], wi.data_ptr(), fp8._DTYPE[wi.dtype], rows, N, K,
+                                              fp8._ptr(off), calls, grads, y.data_ptr(), fp8._ptr(saved), work.data_ptr(), fp8._stream(x)))
+            ctx.save_for_backward(saved, off)
+            ctx.what = (rows, N, K, G, grads, x.dtype, w.dtype, w.shape)
+            return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        offsets, xct, xsf_t, wc, wsf_t = ctx.saved_tensors
-        x_dtype, w_dtype = ctx.dtypes
-        need_x, need_w = ctx.needs_input_grad[:2]
-        gx = gw = None
-        if need_w:
-            gc, gsf, gct, gsf_t = fp8.quantize_fp8_both(gy, offsets, rows_too=need_x)
-        elif need_x:
-            gc, gsf = fp8.quantize_fp8_packed(gy, offsets)
-        out_w = w_dtype if w_dtype in (torch.float32, torch.bfloat16) else torch.float32
-        if offsets is None:
-            gx = fp8.fp8_gemm_nn(gc, wc, gsf, wsf_t, x_dtype) if need_x else None
-            gw = fp8.fp8_gemm_tn(gct, xct, gsf_t, xsf_t, out_w) if need_w else None
-        else:
-            gx = fp8.fp8_gemm_grouped_nn(gc, wc, gsf, wsf_t, offsets, x_dtype) if need_x else None
-            gw = fp8.fp8_gemm_grouped_tn(gct, xct, gsf_t, xsf_t, offsets, ctx.rows, out_w) if need_w else None
-        return gx, (gw.to(w_dtype) if need_w else None), None
+        saved, off = ctx.saved_tensors
+        rows, N, K, G, grads, x_dtype, w_dtype, w_shape = ctx.what
+        with on_device_of(gy, saved, off):
+            gy = fp8._input(gy)
+            dev = gy.device
+            gx = torch.empty((rows, K), dtype=x_dtype, device=dev) if grads & _GRAD_X else None
+            gw = torch.empty(w_shape, dtype=w_dtype if w_dtype in fp8._DTYPE else torch.float32, device=dev) if grads & _GRAD_W else None
+            work = _buffer(_BACKWARD, rows, N, K, G, grads, dev)
+            check(lib().ls_fp8_linear_backward(gy.data_ptr(), fp8._DTYPE[gy.dtype], rows, N, K, fp8._ptr(off), max(G, 1), grads,
+                                               saved.data_ptr(), fp8._ptr(gx), fp8._DTYPE[x_dtype], fp8._ptr(gw),
+                                               _lib.LS_F32 if gw is None else fp8._DTYPE[gw.dtype], work.data_ptr(), fp8._stream(gy)))
+            return gx, (gw if gw is None or gw.dtype == w_dtype else gw.to(w_dtype)), None
 
 
 def linear(x, weight):
     """x [..., in] (bf16 or fp32), weight [out, in] -> [..., out] in x's dtype, with FP8 gradients."""
     _check(x, weight, 2)
-    y = _FP8Matmul.apply(x.reshape(-1, x.shape[-1]), weight, None)
-    return y.view(*x.shape[:-1], weight.shape[0])
-
-
-def linear_quantized(x, codes, sf, out_dtype=None):
-    """linear(x, w) for a weight quantized beforehand (codes and sf of fp8.quantize_fp8_weight); no gradients."""
-    _check(x, codes, 2)
-    xc, xsf = fp8.quantize_fp8_packed(x.reshape(-1, x.shape[-1]))
-    return fp8.fp8_gemm(xc, codes, xsf, sf, out_dtype or x.dtype).view(*x.shape[:-1], codes.shape[0])
+    if x.dim() == 2:
+        return _FP8Matmul.apply(x, weight, None)
+    return _FP8Matmul.apply(x.reshape(-1, x.shape[-1]), weight, None).view(*x.shape[:-1], weight.shape[0])
 
 
 def grouped_linear(x, weight, offsets):
@@ -88,14 +103,37 @@ def grouped_linear(x, weight, offsets):
     return _FP8Matmul.apply(x, weight, offsets)
 
 
+def _serve(x, codes, sf, offsets, out_dtype, out):
+    with on_device_of(x, codes, sf, offsets, out):
+        off, G, calls = _rows_of(x, codes, offsets)
+        x = fp8._aligned(x)
+        (rows, K), N = x.shape, codes.shape[-2]
+        codes, ld = fp8._pitched(codes)
+        sf = fp8._sf(sf, calls * fp8.sf_bytes(N, K), "sf")
+        out_dtype = out_dtype or x.dtype
+        code = fp8._out_code(out_dtype)
+        y = torch.empty((rows, N), dtype=out_dtype, device=x.device) if out is None else fp8._given(out, (rows, N), out_dtype)
+        work = _buffer(_SERVE, rows, N, K, G, 0, x.device)
+        check(lib().ls_fp8_linear(x.data_ptr(), fp8._DTYPE[x.dtype], rows, K, codes.data_ptr(), ld, sf.data_ptr(), N, y.data_ptr(), code,
+                                  fp8._ptr(off), calls, 1 if out is None else 0, work.data_ptr(), fp8._stream(x)))
+        return y
+
+
+def linear_quantized(x, codes, sf, out_dtype=None):
+    """linear(x, w) for a weight quantized beforehand (codes and sf of fp8.quantize_fp8_weight); no gradients."""
+    _check(x, codes, 2)
+    if x.dim() == 2:
+        return _serve(x, codes, sf, None, out_dtype, None)
+    return _serve(x.reshape(-1, x.shape[-1]), codes, sf, None, out_dtype, None).view(*x.shape[:-1], codes.shape[0])
+
+
 def grouped_linear_quantized(x, codes, sf, offsets, out_dtype=None, out=None):
     """grouped_linear for weights quantized beforehand; no gradients.  With `out` the rows of no
     expert are left as they were."""
     _check(x, codes, 3)
     if x.dim() != 2:
         raise ValueError(f"rows sorted by expert are two-dimensional, got shape {tuple(x.shape)}")
-    xc, xsf = fp8.quantize_fp8_packed(x, offsets)
-    return fp8.fp8_gemm_grouped(xc, codes, xsf, sf, offsets, out_dtype or x.dtype, out)
+    return _serve(x, codes, sf, offsets, out_dtype, out)
 
 
 class FP8Linear(nn.Linear):

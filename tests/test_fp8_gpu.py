@@ -210,3 +210,60 @@ def test_grouped_products(sizes, N, K, tail, variant):
         _close(gw[g], *ref.grad_weight(gy[rows], x[rows]), f"gw of group {g}")
     assert (y[at:] == 0).all() and (gx[at:] == 0).all()
     assert torch.equal(kept[:at], y[:at]) and (kept[at:] == 7.0).all()
+
+
+# ---------------------------------------------------------------- layers
+@pytest.mark.parametrize("wdtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,K,N", [(1, 128, 128), (257, 200, 131), (640, 1000, 512)])
+def test_linear_and_gradients(T, K, N, dtype, wdtype):
+    from lockstep_b200 import fp8, fp8_linear
+    x, gy = _data(T, K, seed=11, dtype=dtype), _data(T, N, seed=12, dtype=dtype)
+    w = _data(N, K, seed=13, dtype=wdtype)
+    xi, wi = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = fp8_linear.linear(xi, wi)
+    y.backward(gy)
+    _status()
+    assert y.dtype == dtype and xi.grad.dtype == dtype and wi.grad.dtype == wdtype
+    _close(y.detach(), *ref.forward(x, w), "y")
+    _close(xi.grad, *ref.grad_input(gy, w), "gx")
+    _close(wi.grad, *ref.grad_weight(gy, x), "gw")
+    # one gradient at a time, without gradients, and from quantized weights: the same bits
+    a = torch.autograd.grad(fp8_linear.linear(xi, w), xi, gy)[0]
+    b = torch.autograd.grad(fp8_linear.linear(x, wi), wi, gy)[0]
+    assert torch.equal(a, xi.grad) and torch.equal(b, wi.grad)
+    assert torch.equal(fp8_linear.linear(x, w), y)
+    codes, sf, _ = fp8.quantize_fp8_weight(w)
+    assert torch.equal(fp8_linear.linear_quantized(x, codes, sf), y)
+    x3 = x.view(1, T, 1, K)
+    assert torch.equal(fp8_linear.linear_quantized(x3, codes, sf), y.view(1, T, 1, N))
+    assert torch.equal(fp8_linear.linear(x3, w), y.view(1, T, 1, N))
+
+
+@pytest.mark.parametrize("sizes,tail", [([5, 0, 300, 1], 9), ([0, 0], 3), ([128, 256], 0)])
+def test_grouped_linear_and_gradients(sizes, tail):
+    from lockstep_b200 import fp8, fp8_linear
+    T, G, K, N = sum(sizes) + tail, len(sizes), 200, 136
+    x, gy = _data(T, K, seed=14), _data(T, N, seed=15)
+    layer = fp8_linear.FP8GroupedLinear(G, K, N).cuda()
+    off = _offsets(sizes)
+    xi = x.clone().requires_grad_()
+    y = layer(xi, off)
+    y.backward(gy)
+    _status()
+    at, w = 0, layer.weight.detach()
+    for g, n in enumerate(sizes):
+        rows = slice(at, at + n)
+        at += n
+        if n == 0:
+            assert (layer.weight.grad[g] == 0).all()
+            continue
+        _close(y.detach()[rows], *ref.forward(x[rows], w[g]), "y")
+        _close(xi.grad[rows], *ref.grad_input(gy[rows], w[g]), "gx")
+        _close(layer.weight.grad[g], *ref.grad_weight(gy[rows], x[rows]), "gw")
+    assert (y[at:] == 0).all() and (xi.grad[at:] == 0).all()
+    codes, sf, _ = fp8.quantize_fp8_weight(w)
+    assert torch.equal(fp8_linear.grouped_linear_quantized(x, codes, sf, off), y)
+    kept = torch.full((T, N), 3.0, device="cuda", dtype=x.dtype)
+    assert fp8_linear.grouped_linear_quantized(x, codes, sf, off, out=kept) is kept
+    assert torch.equal(kept[:at], y[:at]) and (kept[at:] == 3.0).all()
