@@ -497,6 +497,10 @@ int ls_fp8_linear_backward(const void *gy, int dtype, int64_t rows, int64_t N, i
                            int64_t groups, int grads, const void *saved, void *gx, int gx_dtype, void *gw,
                            int gw_dtype, void *work, void *stream);
 
+/* For measurements and tests: 0 keeps ls_fp8_linear from taking its one-launch
+ * form for a few rows; 1 (default) lets it choose by size. */
+int ls_fp8_linear_set_skinny(int on);
+
 /* For measurements and tests: 0 = choose by size (default); 1, 3, 4 = one CTA
  * per tile with 128, 64 (form 0 only, else 128), 256 columns; 2 = CTA pairs. */
 int ls_fp8_gemm_set_variant(int variant);

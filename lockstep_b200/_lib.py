@@ -85,6 +85,7 @@ _SIGS = {
     "ls_fp8_linear_forward": (c_int, [c_vp, c_int, c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_int, c_vp, c_vp, c_vp, c_vp]),
     "ls_fp8_linear_backward": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_i64, c_int, c_vp, c_vp, c_int, c_vp, c_int,
                                        c_vp, c_vp]),
+    "ls_fp8_linear_set_skinny": (c_int, [c_int]),
     "ls_fp8_gemm_set_variant": (c_int, [c_int]),
     "ls_scales_to_sf": (c_int, [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "ls_scales_to_sf_block": (c_int, [c_vp, c_i64, c_i64, c_int, c_vp, c_vp, c_vp]),

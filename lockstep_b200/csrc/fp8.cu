@@ -12,57 +12,6 @@
 namespace ls {
 namespace {
 
-constexpr uint32_t kAbs = 0x7FFFFFFFu;
-
-// Values are kept as the 32-bit words they were loaded in: one fp32 value, or two bf16 values.
-// bf16 pairs are handled two at a time: packed NaN-propagating maxima of magnitudes (a 16-bit
-// integer maximum of pairs is several instructions), and scaled by a packed multiplication, which is
-// exact (a power of two; results below bf16's range are far below E4M3's).
-template <typename T> struct Word {
-    static constexpr bool PAIR = sizeof(T) == 2;
-    static constexpr uint32_t MAG = PAIR ? 0x7FFF7FFFu : kAbs;
-    static __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b)   // of magnitudes
-    {
-        if constexpr (!PAIR) return max(a, b);
-        uint32_t m;
-        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
-        return m;
-    }
-    // fp32 bits of the larger half
-    static __device__ __forceinline__ uint32_t fold(uint32_t m) { return PAIR ? max(m & 0xFFFF0000u, m << 16) : m; }
-    // the reciprocal scale as a word that multiplies (both halves of) a word
-    static __device__ __forceinline__ uint32_t inv(uint32_t e8m0)
-    {
-        return PAIR ? ((254u - e8m0) << 7) * 0x00010001u : (254u - e8m0) << 23;
-    }
-    // E4M3 codes of two words of pairs, or four words, times their reciprocal scales
-    static __device__ __forceinline__ uint32_t codes(const uint32_t *w, const uint32_t *inv)
-    {
-        if constexpr (PAIR) {
-            uint32_t q[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(q[i]) : "r"(w[i]), "r"(inv[i]));
-            return cvt_e4m3x4(__uint_as_float(q[0] << 16), __uint_as_float(q[0] & 0xFFFF0000u),
-                              __uint_as_float(q[1] << 16), __uint_as_float(q[1] & 0xFFFF0000u));
-        } else {
-            return cvt_e4m3x4(__uint_as_float(w[0]) * __uint_as_float(inv[0]), __uint_as_float(w[1]) * __uint_as_float(inv[1]),
-                              __uint_as_float(w[2]) * __uint_as_float(inv[2]), __uint_as_float(w[3]) * __uint_as_float(inv[3]));
-        }
-    }
-    // sets a non-finite value to zero and flags it: bit 0 the low half (or the value), bit 1 the high half
-    static __device__ __forceinline__ uint32_t drop_special(uint32_t &w)
-    {
-        uint32_t flags = 0;
-        if constexpr (PAIR) {
-            if ((w & 0x7F80u) == 0x7F80u) flags |= 1u, w &= 0xFFFF0000u;
-            if ((w & 0x7F800000u) == 0x7F800000u) flags |= 2u, w &= 0xFFFFu;
-        } else if ((w & kAbs) >= kBitsInf) {
-            flags = 1u, w = 0u;
-        }
-        return flags;
-    }
-};
-
 // E4M3 has no infinity: non-finite values, whose codes were stored as zeros, become its NaN.
 // Byte stores out of line, so that the ordinary path carries none of it.
 __device__ __noinline__ void store_nans(uint8_t *dst, uint32_t flags)
@@ -77,51 +26,91 @@ __device__ __forceinline__ void ld_stream32(const void *p, uint32_t *w)
                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
 }
 
-// WORDS words of consecutive values from x, of which the first `left` values exist (zeros after them)
-template <int WORDS, typename T>
-__device__ __forceinline__ void load_ragged(const T *x, int left, uint32_t *w)
+// ---- ragged groups ------------------------------------------------------------------------
+// The clamped offsets (groups + 1 of them) in shared memory.  Called by the whole CTA.
+__device__ __forceinline__ void load_bounds(int *bounds, const int *offsets, int groups, int rows)
 {
-#pragma unroll
-    for (int i = 0; i < WORDS; i++) {
-        if constexpr (sizeof(T) == 2) {
-            const uint16_t *h = reinterpret_cast<const uint16_t *>(x);
-            const uint32_t lo = 2 * i < left ? h[2 * i] : 0u, hi = 2 * i + 1 < left ? h[2 * i + 1] : 0u;
-            w[i] = lo | (hi << 16);
-        } else {
-            w[i] = i < left ? __float_as_uint(x[i]) : 0u;
-        }
+    for (int g = threadIdx.x; g <= groups; g += blockDim.x) bounds[g] = group_lo(offsets, g, rows);
+    __syncthreads();
+}
+// Row of x -> its slot row, -1 if it belongs to no group.  Called by a whole warp with one row.
+__device__ __forceinline__ int slot_row(const int *bounds, int groups, int row)
+{
+    const int lane = threadIdx.x & 31;
+    int before = 0;                                         // groups that start at or before the row
+    for (int g0 = 0; g0 < groups; g0 += 32)
+        before += __popc(__ballot_sync(0xFFFFFFFFu, g0 + lane < groups && bounds[min(g0 + lane, groups)] <= row));
+    const int g = before - 1;
+    if (g < 0 || row >= bounds[g + 1]) return -1;
+    return (bounds[g] / 128 + g) * 128 + row - bounds[g];
+}
+// Slot t -> its first row and row count (0: no such tile).  Called by a whole warp.
+__device__ __forceinline__ void slot_rows(const int *bounds, int groups, int t, int &row0, int &n)
+{
+    const int lane = threadIdx.x & 31;
+    int before = 0;                                         // groups whose first slot is at or before t
+    for (int g0 = 0; g0 < groups; g0 += 32) {
+        const int g = g0 + lane;
+        before += __popc(__ballot_sync(0xFFFFFFFFu, g < groups && bounds[min(g, groups)] / 128 + g <= t));
     }
+    const int g = max(before - 1, 0);
+    const int i = t - (bounds[g] / 128 + g);
+    row0 = bounds[g] + 128 * max(i, 0);
+    n = i < 0 ? 0 : max(0, min(128, bounds[g + 1] - row0));
 }
 
-// ---- blocks along the rows of a dense tensor -----------------------------------------------
+// ---- blocks along the rows -----------------------------------------------
 // One warp takes 512 consecutive values of a row = 4 blocks = one scale word; 8 lanes share a block.
+// Rows that do not start on 32-byte boundaries are read element by element, lane by lane along the
+// row, and turned into 16 values per lane through shared memory (each lane's run padded by 16 bytes
+// against bank conflicts).
+template <typename T> constexpr int kTurn = 32 * (16 + 16 / int(sizeof(T)));
+
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_chunk(const T *x, int left, uint32_t (&w)[8 * sizeof(T) / 2])
+__device__ __forceinline__ void load_chunk(const T *row, int chunk, int K, T *turn, uint32_t (&w)[8 * sizeof(T) / 2])
 {
     constexpr int WORDS = 8 * sizeof(T) / 2;
+    const int lane = threadIdx.x & 31;
     if constexpr (VEC) {
+        const int col = chunk * 512 + lane * 16;
 #pragma unroll
         for (int h = 0; h < WORDS / 8; h++) {
-            if (left > 0) ld_stream32(x + 32 / int(sizeof(T)) * h, w + 8 * h);
+            if (col < K) ld_stream32(row + col + 32 / int(sizeof(T)) * h, w + 8 * h);
             else
                 for (int i = 0; i < 8; i++) w[8 * h + i] = 0u;
         }
     } else {
-        load_ragged<WORDS>(x, left, w);
+        constexpr int RUN = 16 + 16 / int(sizeof(T));
+        T v[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int col = chunk * 512 + 32 * j + lane;
+            v[j] = col < K ? row[col] : T(0.0f);
+        }
+        __syncwarp();                                       // the turn buffer has been read
+#pragma unroll
+        for (int j = 0; j < 16; j++) turn[(2 * j + (lane >> 4)) * RUN + (lane & 15)] = v[j];
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < WORDS / 4; h++) {
+            const uint4 q = reinterpret_cast<const uint4 *>(turn + lane * RUN)[h];
+            w[4 * h] = q.x, w[4 * h + 1] = q.y, w[4 * h + 2] = q.z, w[4 * h + 3] = q.w;
+        }
     }
 }
 
 template <typename T>
-__device__ __forceinline__ void quantize_chunk(uint32_t (&w)[8 * sizeof(T) / 2], int64_t row, int chunk, int K, int chunks,
-                                               uint8_t *codes, int64_t ld, float *scale, uint8_t *sf)
+__device__ __forceinline__ void quantize_chunk(uint32_t (&w)[8 * sizeof(T) / 2], int64_t row, int64_t sf_row, int chunk, int K,
+                                               int chunks, uint8_t *codes, int64_t ld, float *scale, uint8_t *sf)
 {
+    if (sf_row < 0) return;                                 // a row of no group
     using W = Word<T>;
     constexpr int WORDS = 8 * sizeof(T) / 2, PER = WORDS / 4;
     const int lane = threadIdx.x & 31, col = chunk * 512 + lane * 16;
     auto largest = [&]() {
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < WORDS; i++) m = W::max_of(m, w[i] & W::MAG);
+        for (int i = 0; i < WORDS; i++) m = W::max_of(m, w[i]);
         return W::fold(m);
     };
     uint32_t amax = largest(), flags = 0;
@@ -147,17 +136,18 @@ __device__ __forceinline__ void quantize_chunk(uint32_t (&w)[8 * sizeof(T) / 2],
         // the four blocks' bytes as one word: lanes 0, 8, 16, 24 put theirs in place
         const uint32_t word = __reduce_or_sync(0xFFFFFFFFu, e8 << (lane & 24));
         if (lane == 0)
-            *reinterpret_cast<uint32_t *>(sf + sf_offset(uint32_t(row), uint32_t(chunk * 4), uint32_t(chunks))) = word;
+            *reinterpret_cast<uint32_t *>(sf + sf_offset(uint32_t(sf_row), uint32_t(chunk * 4), uint32_t(chunks))) = word;
     }
 }
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256, 4)
-fp8_rows_kernel(const T *__restrict__ x, int64_t rows, int K, uint8_t *__restrict__ codes, int64_t ld,
-                float *__restrict__ scale, uint8_t *__restrict__ sf)
+fp8_rows_kernel(const T *__restrict__ x, int64_t rows, int K, const int *__restrict__ offsets, int groups,
+                uint8_t *__restrict__ codes, int64_t ld, float *__restrict__ scale, uint8_t *__restrict__ sf)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int lane = threadIdx.x & 31;
+    __shared__ int bounds[kFp8MaxGroups + 1];
+    if (offsets) load_bounds(bounds, offsets, groups, int(rows));
     const int chunks = (K + 511) / 512;
     // chunk number of this warp, and its step, as (row, chunk of the row)
     const int64_t first = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5), step = int64_t(gridDim.x) * 8;
@@ -169,19 +159,25 @@ fp8_rows_kernel(const T *__restrict__ x, int64_t rows, int K, uint8_t *__restric
         row += row_step, chunk += chunk_step;
         if (chunk >= chunks) chunk -= chunks, row++;
     };
+    __shared__ alignas(16) T turns[VEC ? 1 : 8][VEC ? 1 : kTurn<T>];
+    T *turn = turns[VEC ? 0 : threadIdx.x >> 5];
     // two chunks at a time: the second one's load is in flight while the first is reduced
     while (row < rows) {
         uint32_t a[8 * sizeof(T) / 2], b[8 * sizeof(T) / 2];
         const int64_t row_a = row;
         const int chunk_a = chunk;
-        load_chunk<T, VEC>(x + row * K + chunk * 512 + lane * 16, K - chunk * 512 - lane * 16, a);
+        load_chunk<T, VEC>(x + row * K, chunk, K, turn, a);
         advance();
         const int64_t row_b = row;
         const int chunk_b = chunk;
-        load_chunk<T, VEC>(x + row * K + chunk * 512 + lane * 16, row < rows ? K - chunk * 512 - lane * 16 : 0, b);
+        load_chunk<T, VEC>(x + row * K, chunk, row < rows ? K : 0, turn, b);
         advance();
-        quantize_chunk<T>(a, row_a, chunk_a, K, chunks, codes, ld, scale, sf);
-        if (row_b < rows) quantize_chunk<T>(b, row_b, chunk_b, K, chunks, codes, ld, scale, sf);
+        const int64_t at_a = offsets ? slot_row(bounds, groups, int(row_a)) : row_a;
+        quantize_chunk<T>(a, row_a, at_a, chunk_a, K, chunks, codes, ld, scale, sf);
+        if (row_b < rows) {
+            const int64_t at_b = offsets ? slot_row(bounds, groups, int(row_b)) : row_b;
+            quantize_chunk<T>(b, row_b, at_b, chunk_b, K, chunks, codes, ld, scale, sf);
+        }
     }
 }
 
@@ -208,31 +204,11 @@ struct TileArgs {
     int matrices;                   // kWeight
     uint8_t *codes;                 // row-wise (or weight) codes, pitch ld, in the input's row order
     int64_t ld;
-    float *scale;                   // kRows: [row, column block]; kWeight: [matrix, row block, column block]; or NULL
+    float *scale;                   // kWeight: [matrix, row block, column block], or NULL
     uint8_t *sf;                    // rows = slot rows, blocks along the columns
     uint8_t *codes_t;               // column-wise codes, pitch ld; groups: rows in slot order, zeros after a group's last
     uint8_t *sf_t;                  // rows = columns of x, blocks = row slots
 };
-
-// Slot t -> its first row and row count (0: no such tile).  Called by a whole warp.
-__device__ __forceinline__ void slot_rows(const TileArgs &p, int t, int lane, int &row0, int &n)
-{
-    if (!p.offsets) {
-        row0 = 128 * t, n = min(128, p.rows - row0);
-        return;
-    }
-    int below = 0;                                          // groups whose first slot is at or before t
-    for (int g0 = 0; g0 < p.groups; g0 += 32) {
-        const int g = g0 + lane;
-        const bool at = g < p.groups && group_lo(p.offsets, g, p.rows) / 128 + g <= t;
-        below += __popc(__ballot_sync(0xFFFFFFFFu, at));
-    }
-    const int g = max(below - 1, 0);
-    const int lo = group_lo(p.offsets, g, p.rows), hi = group_hi(p.offsets, g, p.rows, lo);
-    const int i = t - (lo / 128 + g);
-    row0 = lo + 128 * max(i, 0);
-    n = i < 0 ? 0 : max(0, min(128, hi - row0));
-}
 
 // A thread's 4 x 8 values: bf16 as 4 words per row, fp32 as 8.
 template <typename T> struct Piece {
@@ -253,17 +229,17 @@ template <typename T> struct Piece {
     // fp32 bits of the largest magnitude of row i
     __device__ __forceinline__ uint32_t row_max(int i) const
     {
-        uint32_t m = u[i][0] & W::MAG;
+        uint32_t m = u[i][0];
 #pragma unroll
-        for (int w = 1; w < WORDS; w++) m = W::max_of(m, u[i][w] & W::MAG);
+        for (int w = 1; w < WORDS; w++) m = W::max_of(m, u[i][w]);
         return W::fold(m);
     }
     // largest magnitudes of the R rows in word w: one (fp32) or two (bf16) columns
     __device__ __forceinline__ uint32_t col_max(int w) const
     {
-        uint32_t m = u[0][w] & W::MAG;
+        uint32_t m = u[0][w];
 #pragma unroll
-        for (int i = 1; i < R; i++) m = W::max_of(m, u[i][w] & W::MAG);
+        for (int i = 1; i < R; i++) m = W::max_of(m, u[i][w]);
         return m;
     }
 };
@@ -283,6 +259,8 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
     extern __shared__ uint4 ring[];                        // [D][R rows][CH][thread]
     __shared__ uint32_t colpart[WARPS][16 * P::WORDS];        // per warp: the columns' maxima (or, kWeight, one maximum)
     __shared__ uint32_t colinv[16 * P::WORDS];              // reciprocal scales of the columns, as words
+    __shared__ int bounds[MODE & kWeight ? 1 : kFp8MaxGroups + 1];
+    if (!(MODE & kWeight) && p.offsets) load_bounds(bounds, p.offsets, p.groups, p.rows);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int kb = (p.cols + 127) / 128, kt = (kb + 3) / 4;
     const int total = kb * p.slots * (MODE & kWeight ? p.matrices : 1);
@@ -298,7 +276,8 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
     auto place = [&](const Cursor &c, int &t, int64_t &matrix, int &row0, int &n) {
         matrix = MODE & kWeight ? c.rest / p.slots : 0;
         t = MODE & kWeight ? c.rest - int(matrix) * p.slots : c.rest;
-        slot_rows(p, t, lane, row0, n);
+        if (!(MODE & kWeight) && p.offsets) slot_rows(bounds, p.groups, t, row0, n);
+        else row0 = 128 * t, n = min(128, p.rows - row0);
     };
     auto fetch = [&](const Cursor &c, int stage) {          // one commit group per call, empty past the last tile
         if (RING && c.tile < total) {
@@ -421,10 +400,7 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
             const uint32_t e8 = fp8_e8m0(z);
             constexpr int SHARE = 16 / R;                   // lanes that end up with the same row
             const int mine = r0 + 2 * ((lane & 15) / SHARE);
-            if (lane % SHARE == 0 && mine < n) {
-                if (p.sf) p.sf[sf_offset(uint32_t(128 * t + mine), uint32_t(cb), uint32_t(kt))] = uint8_t(e8);
-                if (p.scale) p.scale[int64_t(row0 + mine) * kb + cb] = __uint_as_float(e8 << 23);
-            }
+            if (lane % SHARE == 0 && mine < n) p.sf[sf_offset(uint32_t(128 * t + mine), uint32_t(cb), uint32_t(kt))] = uint8_t(e8);
 #pragma unroll
             for (int i = 0; i < R; i++) {
                 const uint32_t s = W::inv(__shfl_sync(0xFFFFFFFFu, e8, (lane & 16) | (i * SHARE)));
@@ -439,12 +415,12 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
                 for (int w = 0; w < WARPS; w++) a = W::max_of(a, colpart[w][tid]);
                 const int st = (p.slots + 3) / 4;
                 if constexpr (sizeof(T) == 2) {
-                    const uint32_t e0 = fp8_e8m0(a << 16), e1 = fp8_e8m0(a & 0xFFFF0000u);
+                    const uint32_t e0 = fp8_e8m0((a << 16) & kAbs), e1 = fp8_e8m0(a & 0x7FFF0000u);
                     colinv[tid] = (W::inv(e0) & 0xFFFFu) | (W::inv(e1) & 0xFFFF0000u);
                     p.sf_t[sf_offset(uint32_t(cb * 128 + 2 * tid), uint32_t(t), uint32_t(st))] = uint8_t(e0);
                     p.sf_t[sf_offset(uint32_t(cb * 128 + 2 * tid + 1), uint32_t(t), uint32_t(st))] = uint8_t(e1);
                 } else {
-                    const uint32_t e0 = fp8_e8m0(a);
+                    const uint32_t e0 = fp8_e8m0(a & kAbs);
                     colinv[tid] = W::inv(e0);
                     p.sf_t[sf_offset(uint32_t(cb * 128 + tid), uint32_t(t), uint32_t(st))] = uint8_t(e0);
                 }
@@ -552,21 +528,17 @@ extern "C" int ls_quantize_fp8(const void *x, int dtype, int64_t rows, int64_t K
     if (!codes) return fail(LS_EINVAL, "null pointer");
     if (!aligned16(codes) || !aligned16(sf) || !aligned16(scale)) return fail(LS_EALIGN, "codes and scales must be 16-byte aligned");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (offsets) {
-        TileArgs p{int(rows), int(K), offsets, int(groups), int(fp8_slots(rows, groups)), 1, codes, ld, scale, sf, nullptr, nullptr};
-        return launch_tiles<kRows>(x, dtype, p, st);
-    }
     const int64_t warps = rows * ((K + 511) / 512), want = (warps + 7) / 8, most = int64_t(sm_count()) * 4;
     const unsigned grid = unsigned(want < most ? want : most);
     const bool vec = vectorizes(x, dtype, K, 16);
     if (dtype == LS_BF16) {
         const __nv_bfloat16 *xb = static_cast<const __nv_bfloat16 *>(x);
-        if (vec) fp8_rows_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(xb, rows, int(K), codes, ld, scale, sf);
-        else fp8_rows_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(xb, rows, int(K), codes, ld, scale, sf);
+        if (vec) fp8_rows_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(xb, rows, int(K), offsets, int(groups), codes, ld, scale, sf);
+        else fp8_rows_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(xb, rows, int(K), offsets, int(groups), codes, ld, scale, sf);
     } else {
         const float *xf = static_cast<const float *>(x);
-        if (vec) fp8_rows_kernel<float, true><<<grid, 256, 0, st>>>(xf, rows, int(K), codes, ld, scale, sf);
-        else fp8_rows_kernel<float, false><<<grid, 256, 0, st>>>(xf, rows, int(K), codes, ld, scale, sf);
+        if (vec) fp8_rows_kernel<float, true><<<grid, 256, 0, st>>>(xf, rows, int(K), offsets, int(groups), codes, ld, scale, sf);
+        else fp8_rows_kernel<float, false><<<grid, 256, 0, st>>>(xf, rows, int(K), offsets, int(groups), codes, ld, scale, sf);
     }
     LS_LAUNCH_CHECK("fp8_rows_kernel");
     return LS_OK;

@@ -50,6 +50,82 @@ __device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float 
         "mov.b32 %0, {lo, hi};\n}\n" : "=r"(out) : "f"(a), "f"(b), "f"(c), "f"(d));
     return out;
 }
+constexpr uint32_t kAbs = 0x7FFFFFFFu;
+
+// Values are kept as the 32-bit words they were loaded in: one fp32 value, or two bf16 values.
+// bf16 pairs are handled two at a time: packed NaN-propagating maxima of magnitudes (a 16-bit
+// integer maximum of pairs is several instructions), and scaled by a packed multiplication, which is
+// exact (a power of two; results below bf16's range are far below E4M3's).
+template <typename T> struct Word {
+    static constexpr bool PAIR = sizeof(T) == 2;
+    // the larger magnitude (per half), NaN if either is one; the result's sign means nothing
+    static __device__ __forceinline__ uint32_t max_of(uint32_t a, uint32_t b)
+    {
+        uint32_t m;
+        if constexpr (PAIR) asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+        else asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+        return m;
+    }
+    // fp32 bits of the (larger half's) magnitude
+    static __device__ __forceinline__ uint32_t fold(uint32_t m)
+    {
+        return PAIR ? max(m & 0x7FFF0000u, (m << 16) & kAbs) : m & kAbs;
+    }
+    // the reciprocal scale as a word that multiplies (both halves of) a word
+    static __device__ __forceinline__ uint32_t inv(uint32_t e8m0)
+    {
+        return PAIR ? ((254u - e8m0) << 7) * 0x00010001u : (254u - e8m0) << 23;
+    }
+    // E4M3 codes of two words of pairs, or four words, times their reciprocal scales
+    static __device__ __forceinline__ uint32_t codes(const uint32_t *w, const uint32_t *inv)
+    {
+        if constexpr (PAIR) {
+            uint32_t q[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(q[i]) : "r"(w[i]), "r"(inv[i]));
+            return cvt_e4m3x4(__uint_as_float(q[0] << 16), __uint_as_float(q[0] & 0xFFFF0000u),
+                              __uint_as_float(q[1] << 16), __uint_as_float(q[1] & 0xFFFF0000u));
+        } else {
+            return cvt_e4m3x4(__uint_as_float(w[0]) * __uint_as_float(inv[0]), __uint_as_float(w[1]) * __uint_as_float(inv[1]),
+                              __uint_as_float(w[2]) * __uint_as_float(inv[2]), __uint_as_float(w[3]) * __uint_as_float(inv[3]));
+        }
+    }
+    // sets a non-finite value to zero and flags it: bit 0 the low half (or the value), bit 1 the high half
+    static __device__ __forceinline__ uint32_t drop_special(uint32_t &w)
+    {
+        uint32_t flags = 0;
+        if constexpr (PAIR) {
+            if ((w & 0x7F80u) == 0x7F80u) flags |= 1u, w &= 0xFFFF0000u;
+            if ((w & 0x7F800000u) == 0x7F800000u) flags |= 2u, w &= 0xFFFFu;
+        } else if ((w & kAbs) >= kBitsInf) {
+            flags = 1u, w = 0u;
+        }
+        return flags;
+    }
+};
+
+// WORDS words of consecutive values from x, of which the first `left` values exist (zeros after them)
+template <int WORDS, typename T>
+__device__ __forceinline__ void load_ragged(const T *x, int left, uint32_t *w)
+{
+#pragma unroll
+    for (int i = 0; i < WORDS; i++) {
+        if constexpr (sizeof(T) == 2) {
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(x);
+            const uint32_t lo = 2 * i < left ? h[2 * i] : 0u, hi = 2 * i + 1 < left ? h[2 * i + 1] : 0u;
+            w[i] = lo | (hi << 16);
+        } else {
+            w[i] = i < left ? __float_as_uint(x[i]) : 0u;
+        }
+    }
+}
+
+__device__ __forceinline__ int64_t fp8_sf_tiles_dev(int rows, int blocks) { return int64_t((rows + 127) / 128) * ((blocks + 3) / 4); }
 #endif
+
+// y = q(x) w^T for a few rows in one launch (fp8_skinny.cu); arguments as ls_fp8_linear, checked by it
+bool fp8_skinny_fits(int64_t rows, int64_t N, int64_t K, int64_t groups);       // groups = 0: dense
+int fp8_skinny_linear(const void *x, int dtype, int64_t rows, int64_t K, const uint8_t *codes, int64_t ld, const uint8_t *sf, int64_t N,
+                      void *y, int out_dtype, const int *offsets, int64_t groups, int zero_tail, cudaStream_t st);
 
 }  // namespace ls

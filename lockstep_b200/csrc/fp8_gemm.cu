@@ -31,7 +31,10 @@ namespace {
 constexpr int kThreads = 320;
 constexpr int kTmemCols = 512;
 constexpr int kBlock = 128;             // values of K per stage = per scale block
+constexpr int kSegment = 16;            // blocks per accumulation chain of the LONG kernels
 enum Form { NT = 0, NN = 1, TN = 2 };
+
+constexpr int kStagingWords = 32 * 17;  // one epilogue warp's 32 rows x 16 columns, padded against bank conflicts
 
 template <int CTAS, int BN>
 struct Fp8Cfg {
@@ -41,14 +44,15 @@ struct Fp8Cfg {
     static constexpr int B_BYTES = BCOLS * kBlock;
     static constexpr int SFB_TILES = BN >= 128 ? BN / 128 : 1;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES + 2048;       // 512 B of A's scales, 512 SFB_TILES of B's
-    static constexpr int STAGES = BN == 64 ? 8 : CTAS == 2 || BN == 128 ? 6 : 4;
+    static constexpr int STAGES = BN == 64 ? 7 : CTAS == 2 || BN == 128 ? 6 : 4;
     static constexpr int OVL = BN == 256 ? 32 : 0;         // columns that the two accumulators share
     static constexpr int ACC1 = BN - OVL;
     static constexpr int SFA_COL = 2 * BN - OVL, SFB_COL = SFA_COL + 4;
     static_assert(SFB_COL + 4 * SFB_TILES <= kTmemCols, "tensor memory overflow");
-    static constexpr int TAIL = STAGES * STAGE_BYTES;      // barriers, then offsets and tile prefix of the groups
+    static constexpr int TAIL = STAGES * STAGE_BYTES;      // barriers, the groups' tile prefix, the epilogue warps' staging
     static constexpr int LIST = TAIL + 256;
-    static constexpr int SMEM = LIST + 2 * 4 * (kFp8MaxGroups + 2) + 1024;
+    static constexpr int STAGING = LIST + 4 * (kFp8MaxGroups + 4);
+    static constexpr int SMEM = STAGING + 8 * kStagingWords * 4 + 1024;
     static_assert(SMEM <= 227 * 1024, "shared memory overflow");
 };
 
@@ -61,6 +65,7 @@ struct Fp8Params {
     int zero_tail;                 // NT, NN: rows that belong to no group are set to zero
     int sfa_kt, sfb_kt;            // scale tiles along K per 128 rows of A / columns of B
     int sfb_rt;                    // NT, NN: 128-column scale tiles of one group's B
+    int a_bytes;                   // what one load of an A tile delivers
     int *err;
 };
 
@@ -75,6 +80,33 @@ __device__ __forceinline__ uint32_t cluster_ctarank()
     return r;
 }
 
+// Stores a chunk as store_chunk does, for rows that do not start on 16-byte boundaries and for the
+// ragged last columns: 16 columns at a time go through shared memory, so that 16 lanes write
+// adjacent elements of one row.  (Element stores straight from the accumulator layout touch 32 rows
+// per instruction: 16384 x 4097 outputs took 3 times as long.)
+__device__ __forceinline__ void store_ragged(uint32_t *stage, int row_end, int N, void *cbase, bool bf16, int row0, int lane, int col0,
+                                             const uint32_t (&r)[32])
+{
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (row0 >= row_end || col0 + 16 * h >= N) return;        // uniform over the warp
+        __syncwarp();                                              // the staging area has been read
+#pragma unroll
+        for (int j = 0; j < 16; j++) stage[17 * lane + j] = r[16 * h + j];
+        __syncwarp();
+        const int col = col0 + 16 * h + (lane & 15);
+#pragma unroll 4
+        for (int i = 0; i < 16; i++) {                             // rows i and i + 16: different banks
+            const int k = i + (lane & 16), row = row0 + k;
+            const float v = __uint_as_float(stage[17 * k + (lane & 15)]);
+            if (row < row_end && col < N) {
+                if (bf16) static_cast<__nv_bfloat16 *>(cbase)[int64_t(row) * N + col] = __float2bfloat16_rn(v);
+                else static_cast<float *>(cbase)[int64_t(row) * N + col] = v;
+            }
+        }
+    }
+}
+
 // One output tile of the CTA (pair): everything the three roles need.
 struct Item {
     int g;                         // group
@@ -84,7 +116,11 @@ struct Item {
     int slot;                      // this CTA's row tile in A's scale buffer
 };
 
-template <int CTAS, int BN, int FORM>
+// LONG: sums of more than kSegment blocks in fp32 output.  The tensor core's accumulator drops what does
+// not fit as it adds, always in one direction, so the error of one chain grows with its length (relative
+// to 64 bits: 3.4e-7 after 2048 values of K, 3.6e-6 after 16384); the K loop is cut into segments of
+// kSegment blocks, each a chain of its own, that the epilogue adds in registers.
+template <int CTAS, int BN, int FORM, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                 const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb, const Fp8Params p)
@@ -105,8 +141,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     const uint32_t tmem_slot = acc_free_bar + 16u;
     volatile uint32_t *tmem_slot_p = reinterpret_cast<volatile uint32_t *>(gen_base + C::TAIL + 8 * (2 * C::STAGES + 4));
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot_p + 1);
-    int *list_off = reinterpret_cast<int *>(gen_base + C::LIST);       // [groups + 1] clamped offsets
-    int *list_pre = list_off + kFp8MaxGroups + 2;                      // [groups + 1] tiles (of 128 CTAS rows) before a group
+    int *list_pre = reinterpret_cast<int *>(gen_base + C::LIST);       // [groups + 1] tiles (of 128 CTAS rows) before a group
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t cta = CTAS == 2 ? cluster_ctarank() : 0u;
@@ -151,9 +186,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                 if (lane >= o) sum += v;
             }
             if (g < p.groups) {
-                list_off[g] = lo;
                 list_pre[g] = before + sum - own;
-                if (g == p.groups - 1) list_off[p.groups] = hi, list_pre[p.groups] = before + sum;
+                if (g == p.groups - 1) list_pre[p.groups] = before + sum;
             }
             before += __shfl_sync(0xFFFFFFFFu, sum, 31);
         }
@@ -177,7 +211,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             it.row0 = mt * 128 * CTAS + 128 * int(cta);
             it.row_end = p.M;
             it.slot = mt * CTAS + int(cta);
-            const int lo = p.offsets ? list_off[it.g] : 0;
+            const int lo = p.offsets ? group_lo(p.offsets, it.g, p.K) : 0;
             const int hi = p.offsets ? group_hi(p.offsets, it.g, p.K, lo) : p.K;
             it.kb0 = p.offsets ? lo / 128 + it.g : 0;
             it.nkb = (hi - lo + kBlock - 1) / kBlock;
@@ -192,7 +226,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     else b = m - 1;
                 }
                 it.g = a;
-                lo = list_off[a], hi = group_hi(p.offsets, a, p.M, lo), i = mt - list_pre[a];
+                lo = group_lo(p.offsets, a, p.M), hi = group_hi(p.offsets, a, p.M, lo), i = mt - list_pre[a];
             }
             it.row0 = lo + (i * CTAS + int(cta)) * 128;
             it.row_end = hi;
@@ -220,7 +254,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     // CTAS = 2: every load of either CTA completes on CTA 0's barrier
                     const uint32_t bar = CTAS == 2 ? ptx::map_to_cta(full_bar(s), 0) : full_bar(s);
                     if (cta == 0)
-                        ptx::mbar_expect_tx(full_bar(s), CTAS * (C::A_BYTES + C::B_BYTES + (scales ? 512u * (1 + C::SFB_TILES) : 0u)));
+                        ptx::mbar_expect_tx(full_bar(s), CTAS * (p.a_bytes + C::B_BYTES + (scales ? 512u * (1 + C::SFB_TILES) : 0u)));
                     if (A_MN) ptx::tma_load_3d<CTAS>(st, &tm_a, it.row0, kb * kBlock, 0, bar);
                     else ptx::tma_load_3d<CTAS>(st, &tm_a, k * kBlock, it.row0, 0, bar);
                     const uint32_t stb = st + C::A_BYTES;
@@ -260,41 +294,43 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             bool ok = true;
             for (int t = worker; t < items && ok; t += workers) {
                 const Item it = item_of(t);
-                if (it.nkb == 0) continue;                  // an empty group's weight gradient: no sum to take
-                if (C::OVL > 0) {
-                    // the tile before this one has been read out of the columns the two accumulators share
-                    if (lt > 0 && !(ok = ptx::mbar_wait(acc_free_bar, (lt - 1) & 1, abort_flag))) break;
-                } else {
-                    // this accumulator's previous tile (two tiles back) has been read out
-                    if (lt > 1 && !(ok = ptx::mbar_wait(acc_free_bar + 8u * (lt & 1), ((lt >> 1) - 1) & 1, abort_flag))) break;
-                }
-                ptx::tc_fence_after();
-                const uint32_t acc = tmem_base + ((lt & 1) ? C::ACC1 : 0);
                 // a 64-column tile uses one half of a 128-row scale tile: rows 32 c .. + 31 sit in column c
                 const uint32_t sfb_sub = BN >= 128 ? 0u : uint32_t(it.n0 & 127) / 32u;
-                for (int k = 0; k < it.nkb; k++) {
-                    if (!(ok = ptx::mbar_wait(full_bar(s), ph, abort_flag))) break;
-                    ptx::tc_fence_after();
-                    const int kb = it.kb0 + k;
-                    const uint32_t st16 = uint32_t(s) * (C::STAGE_BYTES >> 4);
-                    if (k == 0 || (kb & 3) == 0) {
-#pragma unroll
-                        for (int b = 0; b < 1 + C::SFB_TILES; b++) ptx::tmem_cp_sf<CTAS>(sfa_t + 4 * b, sfdesc0 + st16 + 32 * b);
+                // (an empty group's weight gradient has no blocks: no sum to take)
+                for (int k0 = 0; k0 < it.nkb && ok; k0 += LONG ? kSegment : it.nkb, lt++) {
+                    if (C::OVL > 0) {
+                        // the sum before this one has been read out of the columns the two accumulators share
+                        if (lt > 0 && !(ok = ptx::mbar_wait(acc_free_bar, (lt - 1) & 1, abort_flag))) break;
+                    } else {
+                        // this accumulator's previous sum (two back) has been read out
+                        if (lt > 1 && !(ok = ptx::mbar_wait(acc_free_bar + 8u * (lt & 1), ((lt >> 1) - 1) & 1, abort_flag))) break;
                     }
-                    const uint32_t id = uint32_t(kb & 3);   // byte of the scale column
+                    ptx::tc_fence_after();
+                    const uint32_t acc = tmem_base + ((lt & 1) ? C::ACC1 : 0);
+                    const int k1 = LONG ? min(k0 + kSegment, it.nkb) : it.nkb;
+                    for (int k = k0; k < k1; k++) {
+                        if (!(ok = ptx::mbar_wait(full_bar(s), ph, abort_flag))) break;
+                        ptx::tc_fence_after();
+                        const int kb = it.kb0 + k;
+                        const uint32_t st16 = uint32_t(s) * (C::STAGE_BYTES >> 4);
+                        if (k == 0 || (kb & 3) == 0) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        ptx::mma_mxf8<CTAS>(acc, adesc0 + st16 + A_STEP * j, bdesc0 + st16 + B_STEP * j, idesc | (id << 29) | (id << 4),
-                                            sfa_t + (id << 30), sfb_t + sfb_sub + (id << 30), (k == 0 && j == 0) ? 0u : 1u);
-                    if (CTAS == 2) ptx::tc_commit_pair(empty_bar(s), 3);
-                    else ptx::tc_commit(empty_bar(s));
-                    if (++s == C::STAGES) s = 0, ph ^= 1;
+                            for (int b = 0; b < 1 + C::SFB_TILES; b++) ptx::tmem_cp_sf<CTAS>(sfa_t + 4 * b, sfdesc0 + st16 + 32 * b);
+                        }
+                        const uint32_t id = uint32_t(kb & 3);   // byte of the scale column
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            ptx::mma_mxf8<CTAS>(acc, adesc0 + st16 + A_STEP * j, bdesc0 + st16 + B_STEP * j, idesc | (id << 29) | (id << 4),
+                                                sfa_t + (id << 30), sfb_t + sfb_sub + (id << 30), (k == k0 && j == 0) ? 0u : 1u);
+                        if (CTAS == 2) ptx::tc_commit_pair(empty_bar(s), 3);
+                        else ptx::tc_commit(empty_bar(s));
+                        if (++s == C::STAGES) s = 0, ph ^= 1;
+                    }
+                    if (ok) {
+                        if (CTAS == 2) ptx::tc_commit_pair(acc_full_bar + 8u * (lt & 1), 3);
+                        else ptx::tc_commit(acc_full_bar + 8u * (lt & 1));
+                    }
                 }
-                if (ok) {
-                    if (CTAS == 2) ptx::tc_commit_pair(acc_full_bar + 8u * (lt & 1), 3);
-                    else ptx::tc_commit(acc_full_bar + 8u * (lt & 1));
-                }
-                lt++;
             }
         }
     } else if (warp >= 2) {
@@ -302,6 +338,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         // Warp w reads the tensor-memory lanes of quarter w % 4 and one half of the tile's columns.
         const int q = warp & 3, half = (warp - 2) >> 2;
         const bool bf16 = p.out_bf16 != 0;
+        uint32_t *stage = reinterpret_cast<uint32_t *>(gen_base + C::STAGING) + (warp - 2) * kStagingWords;
+        const bool vec = p.N % (bf16 ? 8 : 4) == 0;
         int lt = 0;
         bool ok = true;
         for (int t = worker; t < items && ok; t += workers) {
@@ -309,24 +347,19 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             constexpr int CH = BN / 64;                     // chunks of 32 columns per warp
             uint8_t *dst = static_cast<uint8_t *>(p.c) + (FORM == TN ? int64_t(it.g) * p.M * p.N * (bf16 ? 2 : 4) : 0);
             const int row = it.row0 + 32 * q;
+            auto emit = [&](int c, const uint32_t (&r)[32]) {
+                const int col0 = it.n0 + 32 * c;
+                if (vec && col0 + 32 <= p.N) store_chunk(it.row_end, p.N, dst, bf16, row, lane, col0, r);
+                else store_ragged(stage, it.row_end, p.N, dst, bf16, row, lane, col0, r);
+            };
             if (it.nkb == 0) {
                 uint32_t z[32];
 #pragma unroll
                 for (int i = 0; i < 32; i++) z[i] = 0u;
 #pragma unroll 1
-                for (int i = 0; i < CH; i++) store_chunk(it.row_end, p.N, dst, bf16, row, lane, it.n0 + 32 * (CH * half + i), z);
+                for (int i = 0; i < CH; i++) emit(CH * half + i, z);
                 continue;
             }
-            if (!(ok = ptx::mbar_wait(acc_full_bar + 8u * (lt & 1), (lt >> 1) & 1, abort_flag))) break;
-            ptx::tc_fence_after();
-            const uint32_t acc = tmem_base + ((lt & 1) ? C::ACC1 : 0) + (uint32_t(32 * q) << 16);
-            // The 32 columns shared by the accumulators are the last chunk of accumulator 0 and the
-            // first of accumulator 1: their owners read them first and then let the next tile's MMAs
-            // start; the other warps do so at once.  Without shared columns a warp frees its
-            // accumulator when its last load has landed.
-            const bool owner = C::OVL > 0 && ((lt & 1) ? half == 0 : half == 1);
-            const int start = (owner && !(lt & 1)) ? CH - 1 : 0;
-            auto chunk = [&](int i) { return CH * half + (C::OVL > 0 ? ((start + i) & (CH - 1)) : i); };
             auto release = [&]() {
                 ptx::tc_fence_before();
                 __syncwarp();
@@ -336,6 +369,53 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     else ptx::mbar_arrive(bar);
                 }
             };
+            // The 32 columns shared by the accumulators are the last chunk of accumulator 0 and the
+            // first of accumulator 1: their owners read them first and then let the next sum's MMAs
+            // start; the other warps do so at once.  Without shared columns a warp frees its
+            // accumulator when its last load has landed.
+            if constexpr (LONG) {
+                float sum[CH][32];
+#pragma unroll
+                for (int c = 0; c < CH; c++)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) sum[c][i] = 0.0f;
+                for (int k0 = 0; k0 < it.nkb && ok; k0 += kSegment, lt++) {
+                    if (!(ok = ptx::mbar_wait(acc_full_bar + 8u * (lt & 1), (lt >> 1) & 1, abort_flag))) break;
+                    ptx::tc_fence_after();
+                    const uint32_t acc = tmem_base + ((lt & 1) ? C::ACC1 : 0) + (uint32_t(32 * q) << 16) + 32 * CH * half;
+                    const bool last_first = C::OVL > 0 && !(lt & 1) && half == 1, owner = C::OVL > 0 && ((lt & 1) ? half == 0 : half == 1);
+                    auto add = [&](int c, float (&to)[32]) {
+                        uint32_t r[32];
+                        ptx::tmem_ld32(acc + 32 * c, r);
+                        ptx::tmem_ld_wait(r);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) to[i] += __uint_as_float(r[i]);
+                    };
+                    if (C::OVL > 0 && !owner) release();
+                    if (last_first) add(CH - 1, sum[CH - 1]), release();
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        if (c < CH - 1 || !last_first) add(c, sum[c]);
+                        if (c == 0 && owner && !last_first) release();
+                    }
+                    if (C::OVL == 0) release();
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int c = 0; c < CH; c++) {
+                    uint32_t r[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) r[i] = __float_as_uint(sum[c][i]);
+                    emit(CH * half + c, r);
+                }
+                continue;
+            }
+            if (!(ok = ptx::mbar_wait(acc_full_bar + 8u * (lt & 1), (lt >> 1) & 1, abort_flag))) break;
+            ptx::tc_fence_after();
+            const uint32_t acc = tmem_base + ((lt & 1) ? C::ACC1 : 0) + (uint32_t(32 * q) << 16);
+            const bool owner = C::OVL > 0 && ((lt & 1) ? half == 0 : half == 1);
+            const int start = (owner && !(lt & 1)) ? CH - 1 : 0;
+            auto chunk = [&](int i) { return CH * half + (C::OVL > 0 ? ((start + i) & (CH - 1)) : i); };
             if (C::OVL > 0 && !owner) release();
             uint32_t ra[32], rb[32];                        // the next chunk's load is in flight while this one is stored
             ptx::tmem_ld32(acc + 32 * chunk(0), ra);
@@ -345,12 +425,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                 if (i + 1 < CH) ptx::tmem_ld32(acc + 32 * chunk(i + 1), rb);
                 else if (C::OVL == 0) release();
                 if (i == 0 && owner) release();
-                store_chunk(it.row_end, p.N, dst, bf16, row, lane, it.n0 + 32 * chunk(i), ra);
+                emit(chunk(i), ra);
                 if (i + 1 < CH) {
                     ptx::tmem_ld_wait(rb);
                     if (i + 2 < CH) ptx::tmem_ld32(acc + 32 * chunk(i + 2), ra);
                     else if (C::OVL == 0) release();
-                    store_chunk(it.row_end, p.N, dst, bf16, row, lane, it.n0 + 32 * chunk(i + 1), rb);
+                    emit(chunk(i + 1), rb);
                 }
             }
             lt++;
@@ -358,7 +438,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         if (FORM != TN && p.offsets && p.zero_tail) {       // rows behind the last group
             const int64_t bytes = int64_t(p.N) * (bf16 ? 2 : 4);
             uint8_t *dst = static_cast<uint8_t *>(p.c);
-            const int first = group_hi(p.offsets, p.groups - 1, p.M, list_off[p.groups - 1]);
+            const int first = group_hi(p.offsets, p.groups - 1, p.M, group_lo(p.offsets, p.groups - 1, p.M));
             for (int r = first + blockIdx.x * 8 + warp - 2; r < p.M; r += gridDim.x * 8) {
                 uint8_t *line = dst + r * bytes;
                 if (bytes % 16 == 0)
@@ -418,7 +498,7 @@ int make_map(CUtensorMap *m, const MapSpec &k)
     return LS_OK;
 }
 
-template <int CTAS, int BN, int FORM>
+template <int CTAS, int BN, int FORM, bool LONG>
 int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa, const CUtensorMap &tsb, const Fp8Params &p,
            int64_t most_tiles, cudaStream_t st)
 {
@@ -437,12 +517,12 @@ int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa,
     cfg.stream = st;
     std::unique_lock<std::mutex> lk(state_mutex());
     if (!resident[dev]) {
-        LS_CUDA(cudaFuncSetAttribute(fp8_gemm_kernel<CTAS, BN, FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        LS_CUDA(cudaFuncSetAttribute(fp8_gemm_kernel<CTAS, BN, FORM, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         int n = sm_count();
         if (CTAS == 2) {
             cfg.gridDim = dim3(unsigned(sm_count() & ~1), 1, 1);
             cfg.attrs = at + 1, cfg.numAttrs = 1;
-            LS_CUDA(cudaOccupancyMaxActiveClusters(&n, fp8_gemm_kernel<CTAS, BN, FORM>, &cfg));
+            LS_CUDA(cudaOccupancyMaxActiveClusters(&n, fp8_gemm_kernel<CTAS, BN, FORM, LONG>, &cfg));
             if (n < 1) return fail(LS_ECUDA, "no CTA pair of the FP8 product fits on this device");
         }
         resident[dev] = n;
@@ -451,7 +531,7 @@ int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa,
     lk.unlock();
     cfg.gridDim = dim3(unsigned(CTAS * workers), 1, 1);
     cfg.attrs = at, cfg.numAttrs = CTAS == 2 ? 2 : 1;
-    LS_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<CTAS, BN, FORM>, ta, tb, tsa, tsb, p));
+    LS_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<CTAS, BN, FORM, LONG>, ta, tb, tsa, tsb, p));
     return LS_OK;
 }
 
@@ -497,34 +577,52 @@ int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t 
     p.sfb_rt = int((N + 127) / 128);
     p.err = err;
 
-    // Which kernel: see the note at choose() below.
+    // Which kernel.  Pairs do the most per byte staged; but while the tiles of a smaller shape all
+    // run at once, the smaller shape has more SMs working: 128 x 64 tiles (K-major B only) if they
+    // fit the SMs, else 128 x 128 if those do, else pairs of 256 x 256 -- unless a group has too few
+    // rows on average to fill more than the first CTA's half of a pair.
     const int variant = g_variant.load(std::memory_order_relaxed);
-    const int64_t rows_per_group = form == TN ? M : M / groups;
-    bool pair = variant ? variant == 2 : rows_per_group > 128;
-    int bn = 256;
-    if (!pair) {
-        bn = variant == 4 ? 256 : 128;
-        if (form == NT && (variant == 3 || (variant == 0 && ((M + 127) / 128 + groups - 1) * ((N + 127) / 128) * 2 <= sm_count()))) bn = 64;
-    }
-    const int64_t tile_rows = pair ? 256 : 128;
-    const int64_t m_tiles = form == TN || !offsets ? (M + tile_rows - 1) / tile_rows : M / tile_rows + groups;
-    const int64_t items = m_tiles * ((N + bn - 1) / bn) * (form == TN ? groups : 1);
+    const int64_t row_groups = form == TN || !offsets ? 1 : groups;
+    auto tiles = [&](int64_t rows, int64_t cols) {
+        const int64_t m = row_groups == 1 ? (M + rows - 1) / rows : M / rows + row_groups;
+        return m * ((N + cols - 1) / cols) * (form == TN ? groups : 1);
+    };
+    bool pair = false;
+    int bn = 128;
+    if (variant) pair = variant == 2, bn = variant == 4 ? 256 : variant == 3 && form == NT ? 64 : 128;
+    else if (form == NT && tiles(128, 64) <= sm_count()) bn = 64;
+    else if (tiles(128, 128) > sm_count()) pair = M > 128 * row_groups;
+    if (pair) bn = 256;
+    const int64_t items = tiles(pair ? 256 : 128, bn);
     if (items > 0x7FFFFFFFll) return fail(LS_EINVAL, "too many output tiles");
     const int64_t a_tiles = fp8_sf_tiles(form == TN ? M : slots * 128, kblocks);
     const int64_t b_tiles = fp8_sf_tiles(N, kblocks) * depth;
     CUtensorMap ta, tb, tsa, tsb;
-    if (int rc = make_map(&ta, {a, a_inner, a_rows, 1, lda, 128, 128, false})) return rc;
+    // With fewer rows than a tile the box of A is no taller than they need: rows outside the tensor
+    // cost more than rows inside it (one row, 4096 x 4096: 14.7 us with 128-row boxes).  The rest of
+    // the stage keeps what shared memory held; an output row depends on its own row of A only.
+    int a_box = 128;
+    if (form != TN)
+        for (a_box = 16; a_box < M && a_box < 128; a_box *= 2) {}
+    p.a_bytes = a_box * kBlock;
+    if (int rc = make_map(&ta, {a, a_inner, a_rows, 1, lda, 128, a_box, false})) return rc;
     if (int rc = make_map(&tb, {b, b_inner, b_rows, depth, ldb, 128, form == NT && bn == 64 ? 64 : 128, false})) return rc;
     if (int rc = make_map(&tsa, {sfa, 128, a_tiles, 1, 512, 128, 1, true})) return rc;
     if (int rc = make_map(&tsb, {sfb, 128, b_tiles, 1, 512, 128, 1, true})) return rc;
-#define LS_FP8_LAUNCH(F)                                                                        \
-    if (form == F) return pair ? launch<2, 256, F>(ta, tb, tsa, tsb, p, items, st)              \
-                        : bn == 256 ? launch<1, 256, F>(ta, tb, tsa, tsb, p, items, st)         \
-                                    : launch<1, 128, F>(ta, tb, tsa, tsb, p, items, st);
-    if (form == NT && bn == 64) return launch<1, 64, NT>(ta, tb, tsa, tsb, p, items, st);
-    LS_FP8_LAUNCH(NT)
-    LS_FP8_LAUNCH(NN)
-    LS_FP8_LAUNCH(TN)
+    const bool many = out_dtype == LS_F32 && kblocks > kSegment;
+#define LS_FP8_LAUNCH(C, B, F) \
+    return many ? launch<C, B, F, true>(ta, tb, tsa, tsb, p, items, st) : launch<C, B, F, false>(ta, tb, tsa, tsb, p, items, st)
+#define LS_FP8_FORM(F)                          \
+    if (form == F) {                            \
+        if (pair) LS_FP8_LAUNCH(2, 256, F);     \
+        if (bn == 256) LS_FP8_LAUNCH(1, 256, F); \
+        LS_FP8_LAUNCH(1, 128, F);               \
+    }
+    if (form == NT && bn == 64) LS_FP8_LAUNCH(1, 64, NT);
+    LS_FP8_FORM(NT)
+    LS_FP8_FORM(NN)
+    LS_FP8_FORM(TN)
+#undef LS_FP8_FORM
 #undef LS_FP8_LAUNCH
     return LS_OK;
 }

@@ -3,10 +3,14 @@
 // again when the call's kernels are done, and `saved`, kept for the backward pass).  A serving call
 // is a few microseconds of device time; separate calls with a buffer for every operand cost 25 us
 // of host time per linear, this form about half.
+#include <atomic>
+
 #include "fp8.cuh"
 
 namespace ls {
 namespace {
+
+std::atomic<int> g_no_skinny{0};
 
 struct Shape {
     int64_t rows, N, K;
@@ -122,6 +126,17 @@ extern "C" int ls_fp8_linear(const void *x, int dtype, int64_t rows, int64_t K, 
     const Shape s{rows, N, K, offsets, groups};
     if (int rc = check_shape(s, 0)) return rc;
     if (rows == 0 || N == 0) return LS_OK;
+    if (dtype != LS_F32 && dtype != LS_BF16) return fail(LS_EINVAL, "unsupported input dtype %d", dtype);
+    if (out_dtype != LS_F32 && out_dtype != LS_BF16) return fail(LS_EINVAL, "unsupported output dtype %d", out_dtype);
+    if (int rc = check_buffer(y, "y")) return rc;
+    // A few rows (per group): one launch that reads the weights once and quantizes x on the fly.
+    if (K > 0 && fp8_skinny_fits(rows, N, K, offsets ? groups : 0) && !g_no_skinny.load(std::memory_order_relaxed)) {
+        if (!x) return fail(LS_EINVAL, "x is null");
+        if (int rc = check_buffer(w_codes, "w_codes")) return rc;
+        if (int rc = check_buffer(w_sf, "w_sf")) return rc;
+        if (ldw < K || ldw % 16) return fail(LS_EINVAL, "row pitch %lld of the weight's codes", (long long)ldw);
+        return fp8_skinny_linear(x, dtype, rows, K, w_codes, ldw, w_sf, N, y, out_dtype, offsets, groups, zero_tail, static_cast<cudaStream_t>(stream));
+    }
     if (int rc = check_buffer(work, "work")) return rc;
     Carver c{static_cast<uint8_t *>(work)};
     const RowOperand q = take_rows(c, s, K);
@@ -169,5 +184,11 @@ extern "C" int ls_fp8_linear_backward(const void *gy, int dtype, int64_t rows, i
     }
     if (grads & kGradW)
         return product(2, b.gt.codes, pitch(N), keep.x.codes, pitch(K), b.gt.sf, keep.x.sf, gw, gw_dtype, N, K, rows, s, 0, stream);
+    return LS_OK;
+}
+
+extern "C" int ls_fp8_linear_set_skinny(int on)
+{
+    g_no_skinny.store(on ? 0 : 1, std::memory_order_relaxed);
     return LS_OK;
 }
