@@ -462,7 +462,8 @@ int ls_dequantize_fp8(const uint8_t *codes, int64_t ld, const float *scale, int6
  *   form 0  C = A[M, K] B[N, K]^T    sfa of A, sfb of B along K       (forward)
  *   form 1  C = A[M, K] B[K, N]      sfb = B's sf_t                   (input gradient)
  *   form 2  C = A[K, M]^T B[K, N]    column-wise operands and sf_t's  (weight gradient)
- * lda, ldb: row pitches in bytes.  Every pointer is 16-byte aligned. */
+ * lda, ldb: row pitches in bytes; whole rows of that length are readable (what
+ * lies behind a row's values does not count).  Every pointer is 16-byte aligned. */
 int ls_fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t ldb, const uint8_t *sfa,
                 const uint8_t *sfb, void *c, int out_dtype, int64_t M, int64_t N, int64_t K, void *stream);
 
@@ -477,7 +478,7 @@ int ls_fp8_gemm_grouped(int form, const uint8_t *a, int64_t lda, const uint8_t *
 
 /* The linear layer in one call per direction, groups = 1 and offsets NULL for a
  * dense one.  `work` and `saved` are buffers of ls_fp8_linear_bytes(what, ...)
- * bytes (groups = 0: dense), 16-byte aligned; work may be reused once the call's
+ * bytes (groups = 0: dense; 0 bytes: NULL will do), 16-byte aligned; work may be reused once the call's
  * kernels are done, saved goes from forward to backward.  grads: 1 = the
  * gradient of x is wanted, 2 = of w (the same value in all calls of a layer).
  *   ls_fp8_linear           y = x w^T for a weight quantized beforehand

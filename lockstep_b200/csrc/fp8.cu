@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(256, 4)
 fp8_rows_kernel(const T *__restrict__ x, int64_t rows, int K, const int *__restrict__ offsets, int groups,
                 uint8_t *__restrict__ codes, int64_t ld, float *__restrict__ scale, uint8_t *__restrict__ sf)
 {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    begin_dependent_launch();
     __shared__ int bounds[kFp8MaxGroups + 1];
     if (offsets) load_bounds(bounds, offsets, groups, int(rows));
     const int chunks = (K + 511) / 512;
@@ -251,7 +251,7 @@ template <typename T, bool VEC, int MODE>
 __global__ void __launch_bounds__(Piece<T>::THREADS, 2)
 fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
 {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    begin_dependent_launch();
     using P = Piece<T>;
     using W = Word<T>;
     constexpr int D = kRing, CH = P::CHUNKS, R = P::R, WARPS = P::THREADS / 32;
@@ -495,9 +495,16 @@ int launch_tile_kernel(const void *x, const TileArgs &p, int64_t tiles, cudaStre
         }
     }
     const int64_t most = int64_t(sm_count()) * 2;
-    fp8_tile_kernel<T, VEC, MODE><<<unsigned(std::min(tiles, most)), Piece<T>::THREADS, ring, st>>>(static_cast<const T *>(x), p);
-    LS_LAUNCH_CHECK("fp8_tile_kernel");
-    return LS_OK;
+    return launch_dependent(fp8_tile_kernel<T, VEC, MODE>, dim3(unsigned(std::min(tiles, most))), Piece<T>::THREADS, ring, st,
+                            static_cast<const T *>(x), p);
+}
+
+template <typename T, bool VEC>
+int launch_rows(const void *x, int64_t rows, int64_t K, const int *offsets, int64_t groups, uint8_t *codes, int64_t ld, float *scale,
+                uint8_t *sf, unsigned grid, cudaStream_t st)
+{
+    return launch_dependent(fp8_rows_kernel<T, VEC>, dim3(grid), 256, 0, st, static_cast<const T *>(x), rows, int(K), offsets, int(groups),
+                            codes, ld, scale, sf);
 }
 
 template <int MODE>
@@ -531,17 +538,11 @@ extern "C" int ls_quantize_fp8(const void *x, int dtype, int64_t rows, int64_t K
     const int64_t warps = rows * ((K + 511) / 512), want = (warps + 7) / 8, most = int64_t(sm_count()) * 4;
     const unsigned grid = unsigned(want < most ? want : most);
     const bool vec = vectorizes(x, dtype, K, 16);
-    if (dtype == LS_BF16) {
-        const __nv_bfloat16 *xb = static_cast<const __nv_bfloat16 *>(x);
-        if (vec) fp8_rows_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(xb, rows, int(K), offsets, int(groups), codes, ld, scale, sf);
-        else fp8_rows_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(xb, rows, int(K), offsets, int(groups), codes, ld, scale, sf);
-    } else {
-        const float *xf = static_cast<const float *>(x);
-        if (vec) fp8_rows_kernel<float, true><<<grid, 256, 0, st>>>(xf, rows, int(K), offsets, int(groups), codes, ld, scale, sf);
-        else fp8_rows_kernel<float, false><<<grid, 256, 0, st>>>(xf, rows, int(K), offsets, int(groups), codes, ld, scale, sf);
-    }
-    LS_LAUNCH_CHECK("fp8_rows_kernel");
-    return LS_OK;
+    if (dtype == LS_BF16)
+        return vec ? launch_rows<__nv_bfloat16, true>(x, rows, K, offsets, groups, codes, ld, scale, sf, grid, st)
+                   : launch_rows<__nv_bfloat16, false>(x, rows, K, offsets, groups, codes, ld, scale, sf, grid, st);
+    return vec ? launch_rows<float, true>(x, rows, K, offsets, groups, codes, ld, scale, sf, grid, st)
+               : launch_rows<float, false>(x, rows, K, offsets, groups, codes, ld, scale, sf, grid, st);
 }
 
 extern "C" int ls_quantize_fp8_both(const void *x, int dtype, int64_t rows, int64_t K, const int *offsets, int64_t groups,

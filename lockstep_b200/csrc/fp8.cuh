@@ -25,6 +25,29 @@ inline int64_t fp8_slots(int64_t rows, int64_t groups) { return rows / 128 + gro
 inline int64_t fp8_sf_tiles(int64_t rows, int64_t blocks) { return ((rows + 127) / 128) * ((blocks + 3) / 4); }
 
 #ifdef __CUDACC__
+// Programmatic dependent launch: every FP8 kernel may be set up under the tail of the kernel before
+// it and lets the next one do the same; it touches memory only after this.
+__device__ __forceinline__ void begin_dependent_launch()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... Params, typename... Args>
+int launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(unsigned(threads), 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at, cfg.numAttrs = 1;
+    LS_CUDA(cudaLaunchKernelEx(&cfg, kernel, Params(args)...));
+    return LS_OK;
+}
+
 __device__ __forceinline__ int group_lo(const int *offsets, int g, int rows) { return min(max(offsets[g], 0), rows); }
 __device__ __forceinline__ int group_hi(const int *offsets, int g, int rows, int lo)
 {

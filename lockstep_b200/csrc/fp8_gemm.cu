@@ -80,30 +80,70 @@ __device__ __forceinline__ uint32_t cluster_ctarank()
     return r;
 }
 
+// 16 lanes write the 32 columns of one row: lane j holds elements 2 j and 2 j + 1 in `word`, dst is
+// element 2 j.  odd: the row starts on an odd element, so the aligned pairs are elements 2 j + 1 and
+// 2 j + 2, and the first and the last element go alone.
+__device__ __forceinline__ void store_pair(uint16_t *dst, uint32_t word, bool odd, int j, int left, bool in)
+{
+    const uint32_t next = odd ? __shfl_down_sync(0xFFFFFFFFu, word, 1, 16) : 0u;
+    const uint32_t pair = odd ? __funnelshift_r(word, next, 16) : word;
+    const int first = 2 * j + odd;
+    if (!in) return;
+    if (first + 1 < left) *reinterpret_cast<uint32_t *>(dst + odd) = pair;
+    else if (first < left) dst[odd] = uint16_t(pair);
+    if (odd && j == 0) dst[0] = uint16_t(word);
+}
+
 // Stores a chunk as store_chunk does, for rows that do not start on 16-byte boundaries and for the
-// ragged last columns: 16 columns at a time go through shared memory, so that 16 lanes write
-// adjacent elements of one row.  (Element stores straight from the accumulator layout touch 32 rows
-// per instruction: 16384 x 4097 outputs took 3 times as long.)
+// ragged last columns, through shared memory: element stores straight from the accumulator layout
+// touch 32 rows per instruction.  bf16: 16 lanes write the 32 columns of a row as aligned pairs.
+// fp32: 16 columns at a time, 16 lanes a row.
 __device__ __forceinline__ void store_ragged(uint32_t *stage, int row_end, int N, void *cbase, bool bf16, int row0, int lane, int col0,
                                              const uint32_t (&r)[32])
 {
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        if (row0 >= row_end || col0 + 16 * h >= N) return;        // uniform over the warp
+    if (row0 >= row_end || col0 >= N) return;                      // uniform over the warp
+    const int j = lane & 15, up = lane & 16;                       // rows i (lanes 0-15) and i + 16: different banks
+    const int left = min(N - col0, 32), rows = row_end - row0 - up;
+    const int64_t at = int64_t(row0 + up) * N + col0;
+    const uint32_t *from = stage + 17 * up + j;
+    if (bf16) {
         __syncwarp();                                              // the staging area has been read
 #pragma unroll
-        for (int j = 0; j < 16; j++) stage[17 * lane + j] = r[16 * h + j];
-        __syncwarp();
-        const int col = col0 + 16 * h + (lane & 15);
-#pragma unroll 4
-        for (int i = 0; i < 16; i++) {                             // rows i and i + 16: different banks
-            const int k = i + (lane & 16), row = row0 + k;
-            const float v = __uint_as_float(stage[17 * k + (lane & 15)]);
-            if (row < row_end && col < N) {
-                if (bf16) static_cast<__nv_bfloat16 *>(cbase)[int64_t(row) * N + col] = __float2bfloat16_rn(v);
-                else static_cast<float *>(cbase)[int64_t(row) * N + col] = v;
-            }
+        for (int i = 0; i < 16; i++) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+            stage[17 * lane + i] = *reinterpret_cast<const uint32_t *>(&h);
         }
+        __syncwarp();
+        uint16_t *dst = static_cast<uint16_t *>(cbase) + at + 2 * j;
+        if (!(N & 1)) {                                            // every row starts on a pair
+            const bool in = 2 * j < left;
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (in && i < rows) *reinterpret_cast<uint32_t *>(dst + i * int64_t(N)) = from[17 * i];
+            return;
+        }
+        // every other row starts on a pair (the same ones in both halves of the warp)
+        if (row0 & 1) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) store_pair(dst + i * int64_t(N), from[17 * i], (i & 1) == 0, j, left, i < rows);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) store_pair(dst + i * int64_t(N), from[17 * i], (i & 1) != 0, j, left, i < rows);
+        }
+        return;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (16 * h >= left) return;
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 16; i++) stage[17 * lane + i] = r[16 * h + i];
+        __syncwarp();
+        uint32_t *dst = static_cast<uint32_t *>(cbase) + at + 16 * h + j;
+        const bool in = 16 * h + j < left;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (in && i < rows) dst[i * int64_t(N)] = from[17 * i];
     }
 }
 
@@ -167,10 +207,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         ptx::tmem_alloc<CTAS>(tmem_slot, kTmemCols);
         ptx::tmem_relinquish<CTAS>();
     }
-    // Programmatic dependent launch: the set-up so far may overlap the kernel before this one;
-    // nothing below may.  Every thread waits (rows of no group are stored without a load).
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // (every thread waits here: rows of no group are stored without a load)
+    begin_dependent_launch();
     if (warp == 2 && p.offsets) {
         const int rows = FORM == TN ? p.K : p.M;
         int before = 0;
@@ -204,9 +242,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     const int items = m_tiles * n_tiles * (FORM == TN ? p.groups : 1);
     auto item_of = [&](int t) {
         Item it;
-        const int mt = t % m_tiles, rest = t / m_tiles;
-        it.n0 = (FORM == TN ? rest % n_tiles : rest) * BN;
         if (FORM == TN) {
+            const int mt = t % m_tiles, rest = t / m_tiles;
+            it.n0 = rest % n_tiles * BN;
             it.g = rest / n_tiles;
             it.row0 = mt * 128 * CTAS + 128 * int(cta);
             it.row_end = p.M;
@@ -216,18 +254,24 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             it.kb0 = p.offsets ? lo / 128 + it.g : 0;
             it.nkb = (hi - lo + kBlock - 1) / kBlock;
         } else {
+            // Group after group (a group's rows and weight are then used up while they are in L2), rows
+            // of tiles inside a column of tiles.
             it.g = 0;
-            int lo = 0, hi = p.M, i = mt;
+            int lo = 0, hi = p.M, i = t, mine = m_tiles;
             if (p.offsets) {
-                int a = 0, b = p.groups - 1;                // last group whose tiles start at or before mt and that has any
+                int a = 0, b = p.groups - 1;                // last group whose tiles start at or before t
                 while (a < b) {
                     const int m = (a + b + 1) >> 1;
-                    if (list_pre[m] <= mt) a = m;
+                    if (list_pre[m] * n_tiles <= t) a = m;
                     else b = m - 1;
                 }
                 it.g = a;
-                lo = group_lo(p.offsets, a, p.M), hi = group_hi(p.offsets, a, p.M, lo), i = mt - list_pre[a];
+                lo = group_lo(p.offsets, a, p.M), hi = group_hi(p.offsets, a, p.M, lo);
+                i = t - list_pre[a] * n_tiles, mine = list_pre[a + 1] - list_pre[a];
             }
+            const int nt = i / mine;
+            i -= nt * mine;
+            it.n0 = nt * BN;
             it.row0 = lo + (i * CTAS + int(cta)) * 128;
             it.row_end = hi;
             it.slot = (p.offsets ? lo / 128 + it.g : 0) + i * CTAS + int(cta);
@@ -577,26 +621,34 @@ int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t 
     p.sfb_rt = int((N + 127) / 128);
     p.err = err;
 
-    // Which kernel.  Pairs do the most per byte staged; but while the tiles of a smaller shape all
-    // run at once, the smaller shape has more SMs working: 128 x 64 tiles (K-major B only) if they
-    // fit the SMs, else 128 x 128 if those do, else pairs of 256 x 256 -- unless a group has too few
-    // rows on average to fill more than the first CTA's half of a pair.
+    // Which kernel.  A pair's 256 x 256 tile and a single CTA's 128 x 128 tile take the same 512 cycles
+    // per block of K (the smaller tile is bound by shared memory: it stages and reads as many bytes for
+    // half the products of an SM), so the shape that needs fewer rounds wins, and the smaller one if
+    // they need the same (shorter epilogue: 2048 x 1024 over 4999 rows 12.6 us against 17.0).  128 x 64
+    // tiles (K-major B only) take 384 cycles: taken if they need a single round.  Groups with few
+    // rows on average leave the second CTA of a pair idle: single CTAs there.
     const int variant = g_variant.load(std::memory_order_relaxed);
     const int64_t row_groups = form == TN || !offsets ? 1 : groups;
     auto tiles = [&](int64_t rows, int64_t cols) {
         const int64_t m = row_groups == 1 ? (M + rows - 1) / rows : M / rows + row_groups;
         return m * ((N + cols - 1) / cols) * (form == TN ? groups : 1);
     };
+    auto rounds = [&](int64_t items, int64_t workers) { return (items + workers - 1) / workers; };
     bool pair = false;
     int bn = 128;
     if (variant) pair = variant == 2, bn = variant == 4 ? 256 : variant == 3 && form == NT ? 64 : 128;
     else if (form == NT && tiles(128, 64) <= sm_count()) bn = 64;
-    else if (tiles(128, 128) > sm_count()) pair = M > 128 * row_groups;
+    else pair = M > 128 * row_groups && rounds(tiles(256, 256), sm_count() / 2) < rounds(tiles(128, 128), sm_count());
     if (pair) bn = 256;
     const int64_t items = tiles(pair ? 256 : 128, bn);
     if (items > 0x7FFFFFFFll) return fail(LS_EINVAL, "too many output tiles");
     const int64_t a_tiles = fp8_sf_tiles(form == TN ? M : slots * 128, kblocks);
     const int64_t b_tiles = fp8_sf_tiles(N, kblocks) * depth;
+    // Filling what lies outside a tensor is slow (a tile whose 128 columns are partly outside takes almost
+    // twice as long), so along M and N the maps reach into the rows' padding: those sums are not stored.
+    // Along K the extent is exact: behind it the operands read as zeros.
+    const int64_t a_extent = form == TN ? std::min(lda, (M + 127) / 128 * 128) : K;
+    const int64_t b_extent = form == NT ? K : std::min(ldb, (N + 127) / 128 * 128);
     CUtensorMap ta, tb, tsa, tsb;
     // With fewer rows than a tile the box of A is no taller than they need: rows outside the tensor
     // cost more than rows inside it (one row, 4096 x 4096: 14.7 us with 128-row boxes).  The rest of
@@ -605,8 +657,8 @@ int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t 
     if (form != TN)
         for (a_box = 16; a_box < M && a_box < 128; a_box *= 2) {}
     p.a_bytes = a_box * kBlock;
-    if (int rc = make_map(&ta, {a, a_inner, a_rows, 1, lda, 128, a_box, false})) return rc;
-    if (int rc = make_map(&tb, {b, b_inner, b_rows, depth, ldb, 128, form == NT && bn == 64 ? 64 : 128, false})) return rc;
+    if (int rc = make_map(&ta, {a, a_extent, a_rows, 1, lda, 128, a_box, false})) return rc;
+    if (int rc = make_map(&tb, {b, b_extent, b_rows, depth, ldb, 128, form == NT && bn == 64 ? 64 : 128, false})) return rc;
     if (int rc = make_map(&tsa, {sfa, 128, a_tiles, 1, 512, 128, 1, true})) return rc;
     if (int rc = make_map(&tsb, {sfb, 128, b_tiles, 1, 512, 128, 1, true})) return rc;
     const bool many = out_dtype == LS_F32 && kblocks > kSegment;

@@ -19,7 +19,7 @@ struct Shape {
     int64_t matrices() const { return groups; }
     int64_t slot_rows() const { return offsets ? 128 * fp8_slots(rows, groups) : rows; }
 };
-int64_t pitch(int64_t n) { return (n + 15) / 16 * 16; }
+int64_t pitch(int64_t n) { return (n + 127) / 128 * 128; }     // whole lines: see _pitch in fp8.py
 int64_t sf_bytes(int64_t rows, int64_t K) { return ls_fp8_sf_bytes(rows, K); }
 
 // Hands out 128-byte aligned pieces of a buffer; with a null buffer it only counts.
@@ -76,6 +76,12 @@ Backward take_backward(Carver &c, const Shape &s, int grads)
     return b;
 }
 
+// A few rows (per group) go through a kernel that needs no buffer.
+bool few_rows(const Shape &s)
+{
+    return s.K > 0 && fp8_skinny_fits(s.rows, s.N, s.K, s.offsets ? s.groups : 0) && !g_no_skinny.load(std::memory_order_relaxed);
+}
+
 int check_shape(const Shape &s, int grads)
 {
     if (int rc = check_device()) return rc;
@@ -110,7 +116,9 @@ extern "C" int64_t ls_fp8_linear_bytes(int what, int64_t rows, int64_t N, int64_
     const Shape s{rows, N, K, groups > 0 ? &some_offsets : nullptr, groups > 0 ? groups : 1};
     Carver c{nullptr};
     switch (what) {
-    case LS_FP8_SERVE: take_rows(c, s, K); break;
+    case LS_FP8_SERVE:
+        if (!few_rows(s)) take_rows(c, s, K);
+        break;
     case LS_FP8_FORWARD: take_forward(c, s, grads); break;
     case LS_FP8_SAVED: take_saved(c, s, grads); break;
     case LS_FP8_BACKWARD: take_backward(c, s, grads); break;
@@ -130,7 +138,7 @@ extern "C" int ls_fp8_linear(const void *x, int dtype, int64_t rows, int64_t K, 
     if (out_dtype != LS_F32 && out_dtype != LS_BF16) return fail(LS_EINVAL, "unsupported output dtype %d", out_dtype);
     if (int rc = check_buffer(y, "y")) return rc;
     // A few rows (per group): one launch that reads the weights once and quantizes x on the fly.
-    if (K > 0 && fp8_skinny_fits(rows, N, K, offsets ? groups : 0) && !g_no_skinny.load(std::memory_order_relaxed)) {
+    if (few_rows(s)) {
         if (!x) return fail(LS_EINVAL, "x is null");
         if (int rc = check_buffer(w_codes, "w_codes")) return rc;
         if (int rc = check_buffer(w_sf, "w_sf")) return rc;

@@ -56,8 +56,7 @@ fp8_skinny_kernel(const T *__restrict__ x, const SkinnyArgs p)
 {
     using W = Word<T>;
     constexpr int WORDS = 16 * int(sizeof(T)) / 4;          // words of 16 values
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    begin_dependent_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int n0 = blockIdx.x * 16 * p.tiles, tiles = min(p.tiles, (p.N - n0 + 15) / 16);
     const int kb_count = (p.K + 127) / 128, kt = (kb_count + 3) / 4;
@@ -261,11 +260,6 @@ size_t tile_bytes(int64_t K) { return 16 * ((K + 511) / 512) * 4 + kWarps * 16 *
 template <typename T, bool VEC>
 int launch(const void *x, const SkinnyArgs &p, cudaStream_t st)
 {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned((p.N + 16 * p.tiles - 1) / (16 * p.tiles)), unsigned(p.offsets ? (p.groups < p.rows ? p.groups : p.rows) : 1), 1);
-    cfg.blockDim = dim3(32 * kWarps, 1, 1);
-    cfg.dynamicSmemBytes = kRingBytes + x_bytes(p.rows, p.K) + p.tiles * tile_bytes(p.K);
-    cfg.stream = st;
     static bool attr_set[64] = {};
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
@@ -276,12 +270,9 @@ int launch(const void *x, const SkinnyArgs &p, cudaStream_t st)
             attr_set[dev] = true;
         }
     }
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at, cfg.numAttrs = 1;
-    LS_CUDA(cudaLaunchKernelEx(&cfg, fp8_skinny_kernel<T, VEC>, static_cast<const T *>(x), p));
-    return LS_OK;
+    const dim3 grid(unsigned((p.N + 16 * p.tiles - 1) / (16 * p.tiles)), unsigned(p.offsets ? std::min(p.groups, p.rows) : 1), 1);
+    return launch_dependent(fp8_skinny_kernel<T, VEC>, grid, 32 * kWarps, kRingBytes + x_bytes(p.rows, p.K) + p.tiles * tile_bytes(p.K), st,
+                            static_cast<const T *>(x), p);
 }
 
 }  // namespace

@@ -8,9 +8,10 @@ for a block of zeros.  The scales being powers of two, division by them is exact
 cores apply them (`tcgen05.mma.kind::mxf8f6f4.block_scale`).  The maximum runs over the finite
 values; infinities and NaNs become E4M3's NaN.
 
-Sizes are free: a ragged end is a short block.  Codes are float8_e4m3fn tensors whose row pitch
-is a multiple of 16 bytes (a view of a wider buffer where the row length is not); `sf` buffers
-hold the scale bytes in the tensor-core layout of fp4.py.
+Sizes are free: a ragged end is a short block.  Codes are float8_e4m3fn tensors; the quantizers lay
+rows out at a pitch of whole 128-byte lines (a view of a wider buffer where the row length is none),
+the products take any pitch that is a multiple of 16 bytes and copy others.  `sf` buffers hold the
+scale bytes in the tensor-core layout of fp4.py.
 
 Ragged groups (rows sorted by expert): `offsets` is a CUDA tensor of groups + 1 integers, rows
 offsets[g] .. offsets[g + 1] belong to group g.  Nothing reads it on the host.  Groups may be
@@ -71,11 +72,13 @@ def _input(x, dims=2):
 
 
 def _pitch(K):
-    return (K + 15) // 16 * 16
+    # whole 128-byte lines: rows that start inside one cost a tensor copy twice the traffic (a weight
+    # gradient of 4999 rows: 22.5 us at a pitch of 2064 and 1008 bytes, 12.6 at 2048 and 1024)
+    return (K + 127) // 128 * 128
 
 
 def _codes(lead, rows, K, device):
-    if K % 16 == 0:
+    if K % 128 == 0:
         return torch.empty((*lead, rows, K), dtype=_CODES, device=device)
     return torch.empty((*lead, rows, _pitch(K)), dtype=_CODES, device=device)[..., :K]
 
@@ -95,8 +98,10 @@ def _pitched(codes):
     if rows == 1 and (ld < K or ld % 16):                     # the pitch of a single row is free
         ld = _pitch(K) if codes.dim() == 2 else 0
     if (codes.stride(-1) == 1 or K <= 1) and ld >= K and ld % 16 == 0 and codes.data_ptr() % 16 == 0 and \
-            (codes.dim() == 2 or codes.shape[0] <= 1 or codes.stride(0) == rows * ld):
+            (codes.dim() == 2 or codes.shape[0] <= 1 or codes.stride(0) == rows * ld) and \
+            (ld == K or codes.untyped_storage().nbytes() >= codes.storage_offset() + codes.numel() // K * ld):
         return codes, ld
+    # (the last test: the products may read the padding of the last row)
     fresh = _codes(codes.shape[:-2], rows, K, codes.device)
     fresh.view(torch.uint8).copy_(codes.view(torch.uint8))
     return fresh, _pitch(K)
@@ -128,7 +133,7 @@ def _quantize_rows(x, offsets, want_scale, want_sf):
         check(lib().ls_quantize_fp8(x.data_ptr(), _DTYPE[x.dtype], rows, K, _ptr(off), G, codes.data_ptr(), _pitch(K),
                                     _ptr(scale), _ptr(sf), _stream(x)))
         if len(shape) != 2:
-            codes = codes.view(shape) if K % 16 == 0 else codes.unflatten(0, shape[:-1]) if len(shape) > 2 else codes[0]
+            codes = codes.view(shape) if codes.is_contiguous() else codes.unflatten(0, shape[:-1]) if len(shape) > 2 else codes[0]
             scale = None if scale is None else scale.view(*shape[:-1], -1)
         return codes, scale, sf
 

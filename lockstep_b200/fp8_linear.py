@@ -37,11 +37,14 @@ def _check(x, w, dims):
 
 @functools.lru_cache(maxsize=4096)
 def _buffer_bytes(what, rows, N, K, groups, grads):
-    return max(16, int(lib().ls_fp8_linear_bytes(what, rows, N, K, groups, grads)))
+    return int(lib().ls_fp8_linear_bytes(what, rows, N, K, groups, grads))
 
 
 def _buffer(what, rows, N, K, groups, grads, device):
-    return torch.empty(_buffer_bytes(what, rows, N, K, groups, grads), dtype=torch.uint8, device=device)
+    n = _buffer_bytes(what, rows, N, K, groups, grads)
+    if n == 0 and what == _SERVE:                              # a few rows need no buffer
+        return None
+    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
 
 
 def _rows_of(x, w, offsets):
@@ -115,7 +118,7 @@ def _serve(x, codes, sf, offsets, out_dtype, out):
         y = torch.empty((rows, N), dtype=out_dtype, device=x.device) if out is None else fp8._given(out, (rows, N), out_dtype)
         work = _buffer(_SERVE, rows, N, K, G, 0, x.device)
         check(lib().ls_fp8_linear(x.data_ptr(), fp8._DTYPE[x.dtype], rows, K, codes.data_ptr(), ld, sf.data_ptr(), N, y.data_ptr(), code,
-                                  fp8._ptr(off), calls, 1 if out is None else 0, work.data_ptr(), fp8._stream(x)))
+                                  fp8._ptr(off), calls, 1 if out is None else 0, fp8._ptr(work), fp8._stream(x)))
         return y
 
 
