@@ -605,7 +605,7 @@ int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t 
     if (lda < a_inner || ldb < b_inner || lda % 16 || ldb % 16)
         return fail(LS_EINVAL, "row pitches must be multiples of 16 and cover a row (lda=%lld, ldb=%lld)", (long long)lda, (long long)ldb);
     int *err = error_word();
-    if (!err) return fail(LS_ECUDA, "could not allocate the device error word");
+    if (!err) return fail(LS_ECUDA, "the device error word is not available");
 
     // Rows (M) or K that the operands hold: with groups the TN operands are in slot order.
     const int64_t slots = offsets ? fp8_slots(form == TN ? K : M, groups) : ((form == TN ? K : M) + 127) / 128;

@@ -963,16 +963,20 @@ int encode_map_3d(void *map, const void *base, int64_t inner, int64_t rows, int6
     return LS_OK;
 }
 
+// One device int per device: a variable of the module, not an allocation, so that the first call of a
+// process may be one that is being captured into a CUDA graph.
+__device__ int g_error_word;
+
 int *error_word()
 {
-    // one device int per device, allocated on first use and kept for the process
     static int *words[64] = {};
     int dev = 0;
     if (current_device(&dev)) return nullptr;
     std::lock_guard<std::mutex> lk(state_mutex());
     if (!words[dev]) {
-        if (cudaMalloc(&words[dev], sizeof(int)) != cudaSuccess) return nullptr;
-        cudaMemset(words[dev], 0, sizeof(int));
+        void *p = nullptr;
+        if (cudaGetSymbolAddress(&p, g_error_word) != cudaSuccess) return nullptr;
+        words[dev] = static_cast<int *>(p);
     }
     return words[dev];
 }
@@ -1015,7 +1019,7 @@ int gemm_fused(int nbatch, const uint8_t *a0, const uint8_t *a1, const uint8_t *
         return fail(LS_EALIGN, "GEMM operands, scale buffers and outputs must be 16-byte aligned");
     const bool caller_err = err != nullptr;
     if (!err) err = error_word();
-    if (!err) return fail(LS_ECUDA, "could not allocate the device error word");
+    if (!err) return fail(LS_ECUDA, "the device error word is not available");
     CUtensorMap ta0, ta1, tb;
     const int variant = g_gemm_variant.load(std::memory_order_relaxed), forced_splits = g_gemm_splits.load(std::memory_order_relaxed);
     const bool pair = variant == 2 || variant == 6 || (variant == 0 && (nbatch == 2 || M > BM));
@@ -1150,7 +1154,7 @@ int gemm_block16(int nbatch, const uint8_t *a0, const uint8_t *a1, const uint8_t
         (nbatch == 2 && (!aligned16(a1) || !aligned16(sfa1) || !aligned16(c1))))
         return fail(LS_EALIGN, "GEMM operands, scale buffers and outputs must be 16-byte aligned");
     int *err = error_word();
-    if (!err) return fail(LS_ECUDA, "could not allocate the device error word");
+    if (!err) return fail(LS_ECUDA, "the device error word is not available");
     CUtensorMap ta0, ta1, tb;
     // as for blocks of 32: CTA pairs for two batches or more than one row tile, else one CTA per
     // tile with a box of A no taller than A (ls_gemm_set_variant 2 / 1, 3, 5 force either)
@@ -1233,7 +1237,7 @@ extern "C" int ls_gemm_status(int *status_host)
 {
     if (int rc = check_device()) return rc;
     int *err = ls::error_word();
-    if (!err) return fail(LS_ECUDA, "could not allocate the device error word");
+    if (!err) return fail(LS_ECUDA, "the device error word is not available");
     int v = 0;
     LS_CUDA(cudaMemcpy(&v, err, sizeof(int), cudaMemcpyDeviceToHost));
     if (v) LS_CUDA(cudaMemset(err, 0, sizeof(int)));

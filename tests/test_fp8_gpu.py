@@ -327,3 +327,343 @@ def test_few_rows_grouped(sizes, tail, K, N):
             _close(y[at:at + n], *ref.forward(x[at:at + n], w[g]), f"group {g}")
         at += n
     assert (y[at:] == 0).all() and torch.equal(kept[:at], y[:at]) and (kept[at:] == 7.0).all()
+
+
+# ---------------------------------------------------------------- refusals
+def test_python_refusals():
+    from lockstep_b200 import fp8, fp8_linear
+    x, w = _data(64, 256), _data(128, 256)
+    xc, xsf = fp8.quantize_fp8_packed(x)
+    wc, wsf, wsf_t = fp8.quantize_fp8_weight(w)
+    w3, w3sf, _ = fp8.quantize_fp8_weight(w[None])
+    off = _offsets([64])
+    bad = [lambda: fp8.fp8_gemm(xc, wc, wsf, wsf[:-1]),                     # scale buffers of the wrong size or type
+           lambda: fp8.fp8_gemm(xc, wc, xsf.float(), wsf),
+           lambda: fp8.fp8_gemm(xc, wc[:, :128], xsf, wsf),                 # K differs
+           lambda: fp8.fp8_gemm(xc[None], wc, xsf, wsf),
+           lambda: fp8.fp8_gemm_grouped(xc, wc, xsf, wsf, off),             # a matrix where a stack is needed
+           lambda: fp8.fp8_gemm_grouped(xc, w3, xsf, w3sf, _offsets([30, 34])),
+           lambda: fp8.fp8_gemm_grouped_tn(xc, xc, xsf, xsf, off, 64),      # not in slot order
+           lambda: fp8.fp8_gemm(xc, wc, xsf, wsf, out=torch.empty(64, 127, device="cuda", dtype=torch.bfloat16)),
+           lambda: fp8.fp8_gemm(xc, wc, xsf, wsf, torch.float32, out=torch.empty(64, 128, device="cuda", dtype=torch.bfloat16)),
+           lambda: fp8.quantize_fp8_both(x[None]), lambda: fp8.quantize_fp8_weight(x[0]),
+           lambda: fp8.quantize_fp8_packed(x, torch.zeros(1026, dtype=torch.int32, device="cuda")),
+           lambda: fp8.quantize_fp8_packed(x, torch.zeros(1, dtype=torch.int32, device="cuda")),
+           lambda: fp8.quantize_fp8_packed(x[None], off),
+           lambda: fp8.dequantize_fp8(xc, torch.ones(64, 3, device="cuda")),
+           lambda: fp8_linear.linear_quantized(x, wc, wsf[1:]),
+           lambda: fp8_linear.grouped_linear(x, w[None], _offsets([30, 34]))]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    for call in (lambda: fp8.quantize_fp8_packed(x, off.float()), lambda: fp8.fp8_gemm(x, wc, xsf, wsf),
+                 lambda: fp8.fp8_gemm(xc, wc, xsf, wsf, torch.float16), lambda: fp8_linear.linear(x.half(), w)):
+        with pytest.raises(TypeError):
+            call()
+    for call in (lambda: fp8.fp8_gemm(xc, wc.cpu(), xsf, wsf), lambda: fp8.quantize_fp8_packed(x, off.cpu())):
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            call()
+    y = fp8_linear.linear(x.clone().requires_grad_(), w)
+    with pytest.raises(RuntimeError):                                       # no second derivative
+        g = torch.autograd.grad(y, y.grad_fn.next_functions[0][0].variable, torch.ones_like(y), create_graph=True)[0]
+        g.sum().backward()
+
+
+def test_abi_refusals():
+    from lockstep_b200._lib import lib, ptr, stream
+    L, buf = lib(), torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    p, odd = ptr(buf), buf[8:].data_ptr()
+    off = _offsets([4])
+    EINVAL, EALIGN = -1, -2
+
+    def gemm(form=0, a=p, lda=128, b=p, ldb=128, sfa=p, sfb=p, c=p, dt=0, M=4, N=4, K=128):
+        return L.ls_fp8_gemm(form, a, lda, b, ldb, sfa, sfb, c, dt, M, N, K, stream())
+    assert gemm(form=3) == gemm(dt=5) == gemm(M=-1) == gemm(K=1 << 31) == EINVAL
+    assert gemm(a=None) == gemm(b=None) == gemm(sfa=None) == gemm(sfb=None) == gemm(c=None) == EINVAL
+    assert gemm(lda=127) == gemm(ldb=120) == gemm(lda=136) == EINVAL
+    assert gemm(a=odd) == gemm(b=odd) == gemm(c=odd) == gemm(sfa=odd) == EALIGN
+    assert gemm(M=0) == gemm(N=0, c=None) == 0                              # nothing to do
+    grouped = lambda off_, G: L.ls_fp8_gemm_grouped(0, p, 128, p, 128, p, p, p, 0, 4, 4, 128, off_, G, 0, stream())
+    assert grouped(None, 1) == grouped(ptr(off), 0) == grouped(ptr(off), 1025) == EINVAL
+
+    def quant(x=p, dt=0, rows=4, K=128, off_=None, G=0, codes=p, ld=128, scale=None, sf=p):
+        return L.ls_quantize_fp8(x, dt, rows, K, off_, G, codes, ld, scale, sf, stream())
+    assert quant(dt=2) == quant(x=None) == quant(codes=None) == quant(ld=120) == quant(rows=-1) == EINVAL
+    assert quant(off_=ptr(off), G=0) == quant(off_=ptr(off), G=2000) == EINVAL
+    assert quant(codes=odd) == quant(sf=odd) == EALIGN
+    both = lambda **k: L.ls_quantize_fp8_both(p, 0, 4, 128, None, 0, k.get("c", p), k.get("s", p), k.get("ct", p), k.get("st", p), 128, stream())
+    assert both(c=None) == both(ct=None) == both(st=None) == EINVAL and both(ct=odd) == EALIGN
+    assert L.ls_quantize_fp8_weight(p, 0, 1025, 4, 128, p, 128, None, p, p, stream()) == EINVAL
+    serve = lambda **k: L.ls_fp8_linear(k.get("x", p), k.get("dt", 0), k.get("rows", 20), 128, k.get("w", p), k.get("ldw", 128), p, 4, k.get("y", p),
+                                        0, None, k.get("G", 1), 0, k.get("work", p), stream())
+    assert serve(work=None) == serve(y=None) == serve(dt=7) == serve(G=0) == serve(G=3) == EINVAL
+    assert serve(rows=2, x=None) == serve(rows=2, ldw=100) == serve(rows=2, w=None) == EINVAL and serve(rows=2, w=odd) == EALIGN
+    assert L.ls_fp8_linear_forward(p, 0, p, 0, 4, 4, 128, None, 1, 3, p, None, p, stream()) == EINVAL       # nowhere to keep
+    assert L.ls_fp8_linear_forward(p, 0, p, 0, 4, 4, 128, None, 1, 4, p, p, p, stream()) == EINVAL
+    assert L.ls_fp8_gemm_set_variant(5) == EINVAL
+    torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------- how tensors come
+def test_strides_offsets_and_alignment():
+    from lockstep_b200 import fp8, fp8_linear
+    base = _data(260, 700, seed=20)
+    w = _data(130, 256, seed=21)
+    codes, sf, _ = fp8.quantize_fp8_weight(w)
+    want = lambda x: fp8_linear.linear_quantized(x.contiguous(), codes, sf)
+    for x in (base[:, 3:259], base[::2, 100:356], base[1:, :256], base.t()[100:356, :200].t()):
+        assert torch.equal(fp8_linear.linear_quantized(x, codes, sf), want(x))
+    # weights at any pitch and alignment
+    x = base[:50, :256].contiguous()
+    wide = torch.zeros(130, 300, dtype=torch.uint8, device="cuda")
+    for at in (0, 16, 5):
+        wide[:, at:at + 256] = codes.view(torch.uint8)
+        view = wide.view(torch.float8_e4m3fn)[:, at:at + 256]
+        assert torch.equal(fp8_linear.linear_quantized(x, view, sf), want(x))
+        assert torch.equal(fp8_linear.linear_quantized(x[:2], view, sf), want(x[:2]))
+    flat = torch.empty(130 * 256 + 7, dtype=torch.uint8, device="cuda")[7:]
+    flat.view(130, 256).copy_(codes.view(torch.uint8))
+    assert torch.equal(fp8_linear.linear_quantized(x, flat.view(130, 256), sf), want(x))
+    # a gradient that is an expanded view
+    xi = x.clone().requires_grad_()
+    fp8_linear.linear(xi, w).sum().backward()
+    ones = torch.ones(50, 130, device="cuda", dtype=torch.bfloat16)
+    _close(xi.grad, *ref.grad_input(ones, w), "gradient of a sum")
+    # the same weight twice in one graph: its gradients add up
+    wi = w.float().requires_grad_()
+    (fp8_linear.linear(x, wi) + fp8_linear.linear(x, wi)).backward(ones)
+    one = torch.autograd.grad(fp8_linear.linear(x, wi), wi, ones)[0]
+    assert torch.equal(wi.grad, one + one)
+
+
+@pytest.mark.parametrize("T,K,N,G", [(0, 64, 64, 0), (5, 64, 0, 0), (5, 0, 64, 0), (0, 64, 64, 3), (6, 0, 32, 2)])
+def test_empty_sizes(T, K, N, G):
+    from lockstep_b200 import fp8_linear
+    x = torch.zeros(T, K, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    w = torch.zeros(*([G] if G else []), N, K, device="cuda", requires_grad=True)
+    off = _offsets([T // 2, T - T // 2] + [0] * (G - 2)) if G else None
+    y = fp8_linear.grouped_linear(x, w, off) if G else fp8_linear.linear(x, w)
+    assert y.shape == (T, N) and (y == 0).all()
+    y.backward(torch.ones_like(y))
+    assert x.grad.shape == x.shape and (x.grad == 0).all() and w.grad.shape == w.shape and (w.grad == 0).all()
+
+
+def test_offsets_out_of_order_stay_in_bounds():
+    # unspecified values, but nothing outside the outputs and no failed wait
+    from lockstep_b200 import fp8, fp8_linear
+    T, K, N = 300, 200, 136
+    x, gy = _data(T, K, seed=22), _data(T, N, seed=23)
+    for vals in ([0, 200, 100, 300], [50, -7, 1 << 30, 20], [-5, -5, -5, -5], [300, 300, 300, 300], [7, 7, 7, 400]):
+        off = torch.tensor(vals, dtype=torch.int32, device="cuda")
+        w = _data(3, N, K, seed=24).requires_grad_()
+        guard = torch.full((T + 64, N), 7.0, device="cuda", dtype=torch.bfloat16)
+        codes, sf, _ = fp8.quantize_fp8_weight(w.detach())
+        fp8_linear.grouped_linear_quantized(x, codes, sf, off, out=guard[32:32 + T])
+        fp8_linear.grouped_linear_quantized(x[:9], codes, sf, off)
+        xi = x.clone().requires_grad_()
+        fp8_linear.grouped_linear(xi, w, off).backward(gy)
+        _status()
+        assert (guard[:32] == 7.0).all() and (guard[32 + T:] == 7.0).all()
+
+
+@pytest.mark.parametrize("M,N", [(300, 513), (7, 130), (129, 64)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_nothing_is_stored_outside_the_output(M, N, out, variant):
+    from lockstep_b200 import fp8
+    x, w = _data(M, 300, seed=25), _data(N, 300, seed=26)
+    xc, xsf = fp8.quantize_fp8_packed(x)
+    wc, wsf, _ = fp8.quantize_fp8_weight(w)
+    flat = torch.full((M * N + 256,), 7.0, device="cuda", dtype=out)
+    c = fp8.fp8_gemm(xc, wc, xsf, wsf, out, out=flat[128:128 + M * N].view(M, N))
+    _close(c, *ref.forward(x, w), "C")
+    assert (flat[:128] == 7.0).all() and (flat[128 + M * N:] == 7.0).all()
+
+
+def test_a_nan_stays_in_its_rows():
+    from lockstep_b200 import fp8, fp8_linear
+    x, w = _data(300, 400, seed=27), _data(200, 400, seed=28)
+    x[17, 3], x[299, 399] = float("nan"), float("-inf")
+    y = fp8_linear.linear(x, w)
+    rows = torch.zeros(300, dtype=torch.bool, device="cuda")
+    rows[17] = rows[299] = True
+    assert y[rows].isnan().all() and y[~rows].isfinite().all()
+    w[5, 0] = float("nan")
+    y = fp8_linear.linear(x, w)
+    assert y[:, 5].isnan().all() and y[~rows][:, [c for c in range(200) if c != 5]].isfinite().all()
+
+
+def test_more_than_2_to_31_values():
+    from lockstep_b200 import fp8
+    rows, K, N = 66000, 33024, 32                              # 2.18e9 values
+    x = torch.empty(rows, K, device="cuda", dtype=torch.bfloat16)
+    x.normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    w = _data(N, K, seed=29)
+    codes, sf = fp8.quantize_fp8_packed(x)
+    wc, wsf, _ = fp8.quantize_fp8_weight(w)
+    y = fp8.fp8_gemm(codes, wc, sf, wsf, torch.float32)
+    _status()
+    for r in (0, 40000, 65409, rows - 1):
+        q, _ = ref.quantize(x[r:r + 1], (1, 128))
+        assert torch.equal(codes[r:r + 1].double(), q)
+        _close(y[r:r + 1], *ref.forward(x[r:r + 1], w), f"row {r}")
+    _, _, codes_t, sf_t = fp8.quantize_fp8_both(x, rows_too=False)
+    q, _ = ref.quantize(x[65920:66000, :300], (128, 1))
+    assert torch.equal(codes_t[65920:, :300].double(), q)
+
+
+# ---------------------------------------------------------------- streams, graphs, threads
+def test_on_another_stream_and_captured():
+    from lockstep_b200 import fp8, fp8_linear
+    w = _data(3, 264, 400, seed=30)
+    codes, sf, _ = fp8.quantize_fp8_weight(w)
+    dense = (codes[0], sf[0].contiguous())
+    runs = {T: (_data(T, 400, seed=31), _offsets([T // 3, 0, T - T // 3])) for T in (3, 200)}
+    calls = [lambda x, o: fp8_linear.linear_quantized(x, *dense), lambda x, o: fp8_linear.grouped_linear_quantized(x, codes, sf, o)]
+    want = {(T, i): f(*a) for T, a in runs.items() for i, f in enumerate(calls)}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = {(T, i): f(*a) for T, a in runs.items() for i, f in enumerate(calls)}
+    side.synchronize()
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    # two graphs of the same calls, replayed in turn and at once, on inputs changed in place
+    graphs = []
+    for _ in range(2):
+        ins = {T: (x.clone(), o.clone()) for T, (x, o) in runs.items()}
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = {(T, i): f(*ins[T]) for T in runs for i, f in enumerate(calls)}
+        graphs.append((g, ins, outs))
+    other = {T: (_data(T, 400, seed=32), _offsets([1, T - 2, 1])) for T in runs}
+    for T in runs:
+        for a, b in zip(graphs[1][1][T], other[T]):
+            a.copy_(b)
+    torch.cuda.synchronize()
+    s0, s1 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(s0):
+            graphs[0][0].replay()
+        with torch.cuda.stream(s1):
+            graphs[1][0].replay()
+    torch.cuda.synchronize()
+    _status()
+    assert all(torch.equal(graphs[0][2][k], want[k]) for k in want)
+    assert all(torch.equal(graphs[1][2][k], calls[k[1]](*other[k[0]])) for k in want)
+
+
+def test_training_step_captured():
+    from lockstep_b200 import fp8_linear
+    x, gy = _data(200, 256, seed=33), _data(200, 136, seed=34)
+    off = _offsets([50, 0, 150])
+    layer = fp8_linear.FP8GroupedLinear(3, 256, 136).cuda()
+    xi = x.clone().requires_grad_()
+    ref_grads = [t.clone() for t in torch.autograd.grad(layer(xi, off), (xi, layer.weight), gy)]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    leaf, weight = x.clone().requires_grad_(), layer.weight.detach().clone().requires_grad_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            torch.autograd.grad(fp8_linear.grouped_linear(leaf, weight, off), (leaf, weight), gy)
+    torch.cuda.current_stream().wait_stream(s)
+    with torch.cuda.graph(g, stream=s):
+        got = torch.autograd.grad(fp8_linear.grouped_linear(leaf, weight, off), (leaf, weight), gy)
+    for t in got:
+        t.zero_()
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], ref_grads[0]) and torch.equal(got[1], ref_grads[1])
+
+
+def test_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    code = ("import torch\nfrom lockstep_b200 import fp8, fp8_linear\n"
+            "x = torch.randn(40, 256, device='cuda').bfloat16(); w = torch.randn(64, 256, device='cuda')\n"
+            "torch.cuda.synchronize(); g = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g):\n    c, s, _ = fp8.quantize_fp8_weight(w); y = fp8_linear.linear_quantized(x, c, s)\n"
+            "g.replay(); torch.cuda.synchronize(); c, s, _ = fp8.quantize_fp8_weight(w)\n"
+            "assert torch.equal(y, fp8_linear.linear_quantized(x, c, s)); print('ok')\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "ok" in r.stdout, r.stderr[-2000:]
+
+
+def test_host_threads_at_once():
+    import threading
+    from lockstep_b200 import fp8, fp8_linear
+    shapes = [(40 + 50 * i, 256 + 64 * i, 136 + 8 * i) for i in range(4)]
+    data = [(_data(T, K, seed=i), fp8.quantize_fp8_weight(_data(N, K, seed=40 + i))) for i, (T, K, N) in enumerate(shapes)]
+    want = [fp8_linear.linear_quantized(x, w[0], w[1]) for x, w in data]
+    torch.cuda.synchronize()
+    fails = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(50):
+                    y = fp8_linear.linear_quantized(data[i][0], data[i][1][0], data[i][1][1])
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(y, want[i]):
+                    fails.append(i)
+        except Exception as e:                                             # noqa: BLE001
+            fails.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    assert not fails, fails
+
+
+# ---------------------------------------------------------------- together, as a model has them
+def test_gradients_against_differences():
+    # linear functionals of y: d/de <c, f(x + e d)> by the operator's own formula; the quantizer is a
+    # staircase, so differences are taken of the unquantized product and must agree with the FP8
+    # gradient within the rounding of its operands (2^-4 relative each, random signs)
+    from lockstep_b200 import fp8_linear
+    x, w, gy = _data(256, 384, seed=35, dtype=torch.float32, spread=0.0), _data(128, 384, seed=36, dtype=torch.float32, spread=0.0), \
+        _data(256, 128, seed=37, dtype=torch.float32, spread=0.0)
+    xi, wi = x.clone().requires_grad_(), w.clone().requires_grad_()
+    fp8_linear.linear(xi, wi).backward(gy)
+    f = lambda a, b: (gy.double() * (a @ b.t())).sum()
+    for got, at in ((xi.grad, 0), (wi.grad, 1)):
+        args = [x.double(), w.double()]
+        d = got.double()                                       # the steepest direction: no cancellation
+        e = 1e-6
+        up, down = list(args), list(args)
+        up[at], down[at] = args[at] + e * d, args[at] - e * d
+        slope = (f(*up) - f(*down)) / (2 * e)
+        assert abs(slope / (d * d).sum() - 1) <= 2.0 ** -4
+
+
+def test_experts_as_a_model_runs_them():
+    # routing -> sort -> grouped up projection -> gelu -> grouped down projection -> unsort, forward and
+    # backward, against the same composition of the oracle's products, step by step
+    from lockstep_b200 import fp8_linear
+    T, G, D, H = 700, 5, 256, 384
+    x, gy = _data(T, D, seed=38, spread=0.3), _data(T, D, seed=39, spread=0.3)
+    up, down = fp8_linear.FP8GroupedLinear(G, D, H).cuda(), fp8_linear.FP8GroupedLinear(G, H, D).cuda()
+    expert = torch.randint(0, G, (T,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    expert[expert == 2] = 3                                    # an expert without rows
+    order = torch.argsort(expert, stable=True)
+    off = torch.cat([torch.zeros(1, device="cuda", dtype=torch.long), torch.bincount(expert, minlength=G).cumsum(0)])
+    xi = x.clone().requires_grad_()
+    h = up(xi[order], off)
+    a = torch.nn.functional.gelu(h)
+    a.retain_grad(), h.retain_grad()
+    y = down(a, off)
+    out = torch.zeros_like(y).index_copy(0, order, y)
+    out.backward(gy)
+    _status()
+    bounds = off.tolist()
+    gs = gy[order]
+    for g in range(G):
+        r = slice(bounds[g], bounds[g + 1])
+        if bounds[g] == bounds[g + 1]:
+            assert (up.weight.grad[g] == 0).all() and (down.weight.grad[g] == 0).all()
+            continue
+        _close(h.detach()[r], *ref.forward(x[order][r], up.weight.detach()[g]), "up")
+        _close(y.detach()[r], *ref.forward(a.detach()[r], down.weight.detach()[g]), "down")
+        _close(a.grad[r], *ref.grad_input(gs[r], down.weight.detach()[g]), "grad of the activation")
+        _close(down.weight.grad[g], *ref.grad_weight(gs[r], a.detach()[r]), "grad of down")
+        _close(up.weight.grad[g], *ref.grad_weight(h.grad[r], x[order][r]), "grad of up")
