@@ -3,7 +3,8 @@
 Sub-modules mirror the reference's module names: fp4, mxfp4_gemm, dual_gemm,
 fp4_linear, wire.  `install_dropins()` registers them under those top-level
 names so that code written against the reference (`import fp4`) runs on this
-package unchanged.
+package unchanged.  Beside them: nvfp4 (the block format lockstep only simulates),
+and fp8 / fp8_linear (E4M3 with one scale per block of 128, dense and grouped by expert).
 """
 
 import importlib

@@ -667,3 +667,22 @@ def test_experts_as_a_model_runs_them():
         _close(a.grad[r], *ref.grad_input(gs[r], down.weight.detach()[g]), "grad of the activation")
         _close(down.weight.grad[g], *ref.grad_weight(gs[r], a.detach()[r]), "grad of down")
         _close(up.weight.grad[g], *ref.grad_weight(h.grad[r], x[order][r]), "grad of up")
+
+
+def test_decoder_steps_with_fp8_projections():
+    # runs, every parameter gets a finite gradient, and the projections' gradients are the operator's
+    import train_bench
+    t = train_bench.Trainer("fp8", layers=2, width=256, heads=4, context=128, batch=4, vocab=512)
+    lin = t.model.blocks[0].attn.proj
+    seen = {}
+    lin.register_forward_hook(lambda m, i, o: (seen.update(x=i[0].detach()), o.register_hook(lambda g: seen.update(gy=g)))[0] and None)
+    t.step()
+    t.flat.zero_()
+    with torch.autocast("cuda", torch.bfloat16):
+        loss = t.model(t.x, t.y)
+    loss.backward()
+    t.close()
+    _status()
+    assert torch.isfinite(loss) and all(p.grad.isfinite().all() for p in t.params)
+    gy, x = seen["gy"].reshape(-1, 256), seen["x"].reshape(-1, 256).bfloat16()
+    _close(lin.weight.grad, *ref.grad_weight(gy, x), "projection weight")

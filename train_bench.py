@@ -12,6 +12,7 @@ The four projections of every block come from `make_linear`:
   "ste"     MXFP4Linear, straight-through bf16 backward        -- lockstep's fp4_linear.py
   "mxfp4"   MXFP4Linear with MXFP4 dgrad / wgrad as well
   "nvfp4"   NVFP4Linear (blocks of 16 under E4M3 scales), straight-through backward
+  "fp8"     FP8Linear (E4M3, one scale per block of 128), dgrad / wgrad in FP8 as well
 
     python train_bench.py --kind mxfp4            # tokens/s
     python train_bench.py --kind mxfp4 --kernels  # device time per kernel of one step
@@ -33,6 +34,9 @@ def make_linear(kind):
         return lambda fan_in, fan_out: nn.Linear(fan_in, fan_out, bias=False)
     if kind == "nvfp4":
         return lambda fan_in, fan_out: fp4_linear.NVFP4Linear(fan_in, fan_out, bias=False)
+    if kind == "fp8":
+        from lockstep_b200 import fp8_linear
+        return lambda fan_in, fan_out: fp8_linear.FP8Linear(fan_in, fan_out, bias=False)
     return lambda fan_in, fan_out: fp4_linear.MXFP4Linear(fan_in, fan_out, bias=False, backward=kind)
 
 
@@ -84,7 +88,7 @@ def make_parts(kind, fused):
     kind "mxfp4" the feed-forward half keeps its activation in MXFP4 between its two GEMMs."""
     from lockstep_b200 import fp4_linear
     linear = make_linear(kind)
-    if fused and kind not in ("dense", "nvfp4"):
+    if fused and kind not in ("dense", "nvfp4", "fp8"):
         return (linear,
                 lambda width, out: fp4_linear.MXFP4NormLinear(width, out, backward=kind),
                 lambda width: fp4_linear.MXFP4MLP(width, 4 * width, backward=kind, norm=True))
@@ -297,7 +301,7 @@ def kernel_table(kind="mxfp4", fused=True, steps=3, top=24, device=None):
 if __name__ == "__main__":
     import argparse
     ap = argparse.ArgumentParser(description="tokens/s of the 12-layer configuration, or the kernel list of one step")
-    ap.add_argument("--kind", default="mxfp4", choices=["dense", "ste", "mxfp4", "nvfp4"])
+    ap.add_argument("--kind", default="mxfp4", choices=["dense", "ste", "mxfp4", "nvfp4", "fp8"])
     ap.add_argument("--unfused", action="store_true", help="separate LayerNorm, GELU and quantizer passes")
     ap.add_argument("--kernels", action="store_true", help="print device time per kernel of one step instead")
     ap.add_argument("--steps", type=int, default=5)
