@@ -131,6 +131,7 @@ def need_cuda(*tensors):
 
 
 _HERE = contextlib.nullcontext()
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)     # without the wrapper's checks
 
 
 def on_device_of(first, *others):
@@ -143,7 +144,7 @@ def on_device_of(first, *others):
             raise RuntimeError(f"lockstep_b200: tensors on different devices ({first.device} and {t.device})")
     if d < 0:
         need_cuda(first)
-    return _HERE if torch.cuda.current_device() == d else torch.cuda.device(d)
+    return _HERE if current_device() == d else torch.cuda.device(d)
 
 
 def aligned(t, n=16):

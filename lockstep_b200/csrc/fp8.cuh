@@ -131,6 +131,15 @@ template <typename T> struct Word {
 template <int WORDS, typename T>
 __device__ __forceinline__ void load_ragged(const T *x, int left, uint32_t *w)
 {
+    if (sizeof(T) == 2 && (reinterpret_cast<uintptr_t>(x) & 3) == 0) {     // pairs on word boundaries
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) {
+            w[i] = 0u;
+            if (2 * i + 1 < left) w[i] = reinterpret_cast<const uint32_t *>(x)[i];
+            else if (2 * i < left) w[i] = reinterpret_cast<const uint16_t *>(x)[2 * i];
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < WORDS; i++) {
         if constexpr (sizeof(T) == 2) {

@@ -31,7 +31,7 @@ namespace {
 constexpr int kThreads = 320;
 constexpr int kTmemCols = 512;
 constexpr int kBlock = 128;             // values of K per stage = per scale block
-constexpr int kSegment = 16;            // blocks per accumulation chain of the LONG kernels
+constexpr int kSegment = 32;            // blocks per accumulation chain of the LONG kernels
 enum Form { NT = 0, NN = 1, TN = 2 };
 
 constexpr int kStagingWords = 32 * 17;  // one epilogue warp's 32 rows x 16 columns, padded against bank conflicts
@@ -158,8 +158,10 @@ struct Item {
 
 // LONG: sums of more than kSegment blocks in fp32 output.  The tensor core's accumulator drops what does
 // not fit as it adds, always in one direction, so the error of one chain grows with its length (relative
-// to 64 bits: 3.4e-7 after 2048 values of K, 3.6e-6 after 16384); the K loop is cut into segments of
-// kSegment blocks, each a chain of its own, that the epilogue adds in registers.
+// to 64 bits: 3.4e-7 after 2048 values of K, 3.6e-6 after 16384).  The K loop is cut into segments of
+// kSegment blocks, each a chain of its own, that the epilogue adds in registers: 2.2e-7 after 16384
+// (torch's fp32 product: 3.6e-7) in 54 us for 4096 x 1024 outputs; segments half as long give 1.2e-7
+// in 57 us, one chain takes 51 us.
 template <int CTAS, int BN, int FORM, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
@@ -579,7 +581,7 @@ int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa,
     return LS_OK;
 }
 
-std::atomic<int> g_variant{0};          // 0 = choose by size; 1 / 2 = single CTA (128 columns) / CTA pair; 3, 4 = single CTA with 64, 256 columns
+std::atomic<int> g_variant{0};          // 0 = choose by size; else see ls_fp8_gemm_set_variant
 
 int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t ldb, const uint8_t *sfa, const uint8_t *sfb,
              void *c, int out_dtype, int64_t M, int64_t N, int64_t K, const int *offsets, int64_t groups, int zero_tail,
@@ -621,26 +623,33 @@ int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t 
     p.sfb_rt = int((N + 127) / 128);
     p.err = err;
 
-    // Which kernel.  A pair's 256 x 256 tile and a single CTA's 128 x 128 tile take the same 512 cycles
-    // per block of K (the smaller tile is bound by shared memory: it stages and reads as many bytes for
-    // half the products of an SM), so the shape that needs fewer rounds wins, and the smaller one if
-    // they need the same (shorter epilogue: 2048 x 1024 over 4999 rows 12.6 us against 17.0).  128 x 64
-    // tiles (K-major B only) take 384 cycles: taken if they need a single round.  Groups with few
-    // rows on average leave the second CTA of a pair idle: single CTAs there.
+    // Which kernel: the one with the smallest product of rounds over the SMs and cycles per block of K.
+    // A pair's 256 x 256 tile takes the tensor cores' 512 cycles.  The tiles of single CTAs are bound by
+    // shared memory, which is written and read once per staged byte at 128 bytes per cycle: 128 x 256
+    // 768, 128 x 128 512, 128 x 64 (K-major B only) 384.  Among equals the smaller tile, whose epilogue is
+    // shorter (2048 x 1024 over 4999 rows: 12.6 us against 17.0 of the pair's).  A ragged group ends in
+    // half a tile on average.  With few rows per group the second CTA of a pair idles: no pairs there.
     const int variant = g_variant.load(std::memory_order_relaxed);
-    const int64_t row_groups = form == TN || !offsets ? 1 : groups;
-    auto tiles = [&](int64_t rows, int64_t cols) {
-        const int64_t m = row_groups == 1 ? (M + rows - 1) / rows : M / rows + row_groups;
+    const bool by_rows = form != TN && offsets;
+    auto tiles = [&](int64_t rows, int64_t cols, int64_t part) {       // part / 2 of a tile more per group
+        const int64_t m = by_rows ? M / rows + (part * groups + 1) / 2 : (M + rows - 1) / rows;
         return m * ((N + cols - 1) / cols) * (form == TN ? groups : 1);
     };
-    auto rounds = [&](int64_t items, int64_t workers) { return (items + workers - 1) / workers; };
-    bool pair = false;
-    int bn = 128;
-    if (variant) pair = variant == 2, bn = variant == 4 ? 256 : variant == 3 && form == NT ? 64 : 128;
-    else if (form == NT && tiles(128, 64) <= sm_count()) bn = 64;
-    else pair = M > 128 * row_groups && rounds(tiles(256, 256), sm_count() / 2) < rounds(tiles(128, 128), sm_count());
-    if (pair) bn = 256;
-    const int64_t items = tiles(pair ? 256 : 128, bn);
+    bool pair = variant == 2;
+    int bn = variant == 4 || variant == 2 ? 256 : variant == 3 && form == NT ? 64 : 128;
+    if (variant == 0) {
+        int64_t best = -1;
+        auto consider = [&](bool p2, int cols, int64_t cycles) {
+            const int64_t workers = p2 ? sm_count() / 2 : sm_count();
+            const int64_t cost = (tiles(p2 ? 256 : 128, cols, 1) + workers - 1) / workers * cycles;
+            if (best < 0 || cost < best) best = cost, pair = p2, bn = cols;
+        };
+        if (form == NT) consider(false, 64, 384);
+        consider(false, 128, 512);
+        consider(false, 256, 768);
+        if (M > (by_rows ? 128 * groups : 128)) consider(true, 256, 512);
+    }
+    const int64_t items = tiles(pair ? 256 : 128, bn, 2);
     if (items > 0x7FFFFFFFll) return fail(LS_EINVAL, "too many output tiles");
     const int64_t a_tiles = fp8_sf_tiles(form == TN ? M : slots * 128, kblocks);
     const int64_t b_tiles = fp8_sf_tiles(N, kblocks) * depth;

@@ -89,6 +89,8 @@ def _bytes(n, device):
 
 def _pitched(codes):
     """(codes, row pitch) as the products read them: rows 16-byte aligned, matrices back to back."""
+    if codes.dtype is _CODES and codes.is_contiguous() and codes.shape[-1] % 16 == 0 and codes.data_ptr() % 16 == 0:
+        return codes, codes.shape[-1]
     if codes.dtype != _CODES:
         if codes.dtype != torch.uint8:
             raise TypeError(f"codes must be float8_e4m3fn (or their bytes), got {codes.dtype}")

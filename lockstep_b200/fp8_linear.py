@@ -44,22 +44,16 @@ def _buffer(what, rows, N, K, groups, grads, device):
     n = _buffer_bytes(what, rows, N, K, groups, grads)
     if n == 0 and what == _SERVE:                              # a few rows need no buffer
         return None
-    return torch.empty(max(n, 16), dtype=torch.uint8, device=device)
-
-
-def _rows_of(x, w, offsets):
-    """(int32 offsets or None, groups as the sizes count them, as the calls do) after checking them against w."""
-    off, G = fp8._groups(offsets)
-    if off is not None and w.shape[0] != G:
-        raise ValueError(f"{w.shape[0]} experts for offsets of {G} groups")
-    return off, G, max(G, 1)
+    return torch.empty((max(n, 16),), dtype=torch.uint8, device=device)
 
 
 class _FP8Matmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
         with on_device_of(x, w, offsets):
-            off, G, calls = _rows_of(x, w, offsets)
+            off, G = fp8._groups(offsets)
+            if off is not None and w.shape[0] != G:
+                raise ValueError(f"{w.shape[0]} experts for offsets of {G} groups")
             xi, wi = fp8._aligned(x), fp8._input(w, w.dim())
             (rows, K), N, dev = xi.shape, w.shape[-2], x.device
             grads = (_GRAD_X if ctx.needs_input_grad[0] else 0) | (_GRAD_W if ctx.needs_input_grad[1] else 0)
@@ -67,7 +61,7 @@ class _FP8Matmul(torch.autograd.Function):
             work = _buffer(_FORWARD, rows, N, K, G, grads, dev)
             saved = _buffer(_SAVED, rows, N, K, G, grads, dev) if grads else None
             check(lib().ls_fp8_linear_forward(xi.data_ptr(), fp8._DTYPE[xi.dtype], wi.data_ptr(), fp8._DTYPE[wi.dtype], rows, N, K,
-                                              fp8._ptr(off), calls, grads, y.data_ptr(), fp8._ptr(saved), work.data_ptr(), fp8._stream(x)))
+                                              fp8._ptr(off), G or 1, grads, y.data_ptr(), fp8._ptr(saved), work.data_ptr(), fp8._stream(x)))
             ctx.save_for_backward(saved, off)
             ctx.what = (rows, N, K, G, grads, x.dtype, w.dtype, w.shape)
             return y
@@ -83,7 +77,7 @@ class _FP8Matmul(torch.autograd.Function):
             gx = torch.empty((rows, K), dtype=x_dtype, device=dev) if grads & _GRAD_X else None
             gw = torch.empty(w_shape, dtype=w_dtype if w_dtype in fp8._DTYPE else torch.float32, device=dev) if grads & _GRAD_W else None
             work = _buffer(_BACKWARD, rows, N, K, G, grads, dev)
-            check(lib().ls_fp8_linear_backward(gy.data_ptr(), fp8._DTYPE[gy.dtype], rows, N, K, fp8._ptr(off), max(G, 1), grads,
+            check(lib().ls_fp8_linear_backward(gy.data_ptr(), fp8._DTYPE[gy.dtype], rows, N, K, fp8._ptr(off), G or 1, grads,
                                                saved.data_ptr(), fp8._ptr(gx), fp8._DTYPE[x_dtype], fp8._ptr(gw),
                                                _lib.LS_F32 if gw is None else fp8._DTYPE[gw.dtype], work.data_ptr(), fp8._stream(gy)))
             return gx, (gw if gw is None or gw.dtype == w_dtype else gw.to(w_dtype)), None
@@ -103,22 +97,31 @@ def grouped_linear(x, weight, offsets):
     _check(x, weight, 3)
     if x.dim() != 2:
         raise ValueError(f"rows sorted by expert are two-dimensional, got shape {tuple(x.shape)}")
+    if offsets is None:
+        raise ValueError("offsets are needed")
     return _FP8Matmul.apply(x, weight, offsets)
 
 
+# One token's linear is a few microseconds on the device, so these two keep to what the call needs;
+# whatever is not the ordinary case goes through the same helpers as everywhere else.
 def _serve(x, codes, sf, offsets, out_dtype, out):
     with on_device_of(x, codes, sf, offsets, out):
-        off, G, calls = _rows_of(x, codes, offsets)
-        x = fp8._aligned(x)
-        (rows, K), N = x.shape, codes.shape[-2]
+        off, G = (None, 0) if offsets is None else fp8._groups(offsets)
+        if off is not None and codes.shape[0] != G:
+            raise ValueError(f"{codes.shape[0]} experts for offsets of {G} groups")
+        if not x.is_contiguous() or x.data_ptr() % 32:
+            x = fp8._aligned(x)
+        rows, K = x.shape
+        N = codes.shape[-2]
         codes, ld = fp8._pitched(codes)
-        sf = fp8._sf(sf, calls * fp8.sf_bytes(N, K), "sf")
-        out_dtype = out_dtype or x.dtype
+        sf = fp8._sf(sf, (G or 1) * fp8.sf_bytes(N, K), "sf")
+        if out_dtype is None:
+            out_dtype = x.dtype
         code = fp8._out_code(out_dtype)
-        y = torch.empty((rows, N), dtype=out_dtype, device=x.device) if out is None else fp8._given(out, (rows, N), out_dtype)
+        y = x.new_empty((rows, N), dtype=out_dtype) if out is None else fp8._given(out, (rows, N), out_dtype)
         work = _buffer(_SERVE, rows, N, K, G, 0, x.device)
         check(lib().ls_fp8_linear(x.data_ptr(), fp8._DTYPE[x.dtype], rows, K, codes.data_ptr(), ld, sf.data_ptr(), N, y.data_ptr(), code,
-                                  fp8._ptr(off), calls, 1 if out is None else 0, fp8._ptr(work), fp8._stream(x)))
+                                  fp8._ptr(off), G or 1, 1 if out is None else 0, fp8._ptr(work), fp8._stream(x)))
         return y
 
 
@@ -136,6 +139,8 @@ def grouped_linear_quantized(x, codes, sf, offsets, out_dtype=None, out=None):
     _check(x, codes, 3)
     if x.dim() != 2:
         raise ValueError(f"rows sorted by expert are two-dimensional, got shape {tuple(x.shape)}")
+    if offsets is None:
+        raise ValueError("offsets are needed")
     return _serve(x, codes, sf, offsets, out_dtype, out)
 
 
