@@ -30,11 +30,11 @@ int gemm_common(int nbatch, const uint8_t *a0, const uint8_t *a1, const uint8_t 
                 const uint8_t *sfa1, const uint8_t *sfb, void *c0, void *c1, int out_dtype, int64_t M,
                 int64_t N, int64_t K, void *stream, int *err);
 
-// Tensor map over [depth][rows][inner]: bytes with the 128-byte swizzle, or (words) 32-bit words
-// unswizzled.  `inner` and `box_inner` count elements, `pitch` bytes between rows; what lies
-// outside the tensor reads as zero.
+// Tensor map over [depth][rows][inner].  `inner` and `box_inner` count elements, `pitch` bytes between
+// rows; what lies outside the tensor reads as zero and is not written.
+enum MapType { kMapBytes, kMapWords, kMapBf16, kMapF32 };     // 32-bit words are unswizzled, the others have the 128-byte swizzle
 int encode_map_3d(void *map, const void *base, int64_t inner, int64_t rows, int64_t depth, int64_t pitch, int box_inner,
-                  int box_rows, bool words);
+                  int box_rows, MapType type);
 int *error_word();                                  // device int of the current device that ls_gemm_status reads; NULL on failure
 
 #define LS_CUDA(expr)                                                              \

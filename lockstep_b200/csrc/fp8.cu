@@ -51,7 +51,7 @@ __device__ __forceinline__ void slot_rows(const int *bounds, int groups, int t, 
     int before = 0;                                         // groups whose first slot is at or before t
     for (int g0 = 0; g0 < groups; g0 += 32) {
         const int g = g0 + lane;
-        before += __popc(__ballot_sync(0xFFFFFFFFu, g < groups && bounds[min(g, groups)] / 128 + g <= t));
+        before += __popc(__ballot_sync(0xFFFFFFFFu, g < groups && (uint32_t(bounds[min(g, groups)]) >> 7) + g <= t));
     }
     const int g = max(before - 1, 0);
     const int i = t - (bounds[g] / 128 + g);
@@ -273,6 +273,7 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
         c.tile += gridDim.x, c.rest += rest_step, c.cb += cb_step;
         if (c.cb >= kb) c.cb -= kb, c.rest++;
     };
+    __shared__ int2 found[P::THREADS / 32][D];              // per warp: rows of the tiles in the ring
     auto place = [&](const Cursor &c, int &t, int64_t &matrix, int &row0, int &n) {
         matrix = MODE & kWeight ? c.rest / p.slots : 0;
         t = MODE & kWeight ? c.rest - int(matrix) * p.slots : c.rest;
@@ -284,6 +285,7 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
             int t, row0, n;
             int64_t matrix;
             place(c, t, matrix, row0, n);
+            if (!(MODE & kWeight) && p.offsets && lane == 0) found[warp][stage] = make_int2(row0, n);   // (searched for once)
             const int col = c.cb * 128 + c0;
             const T *src = x + (matrix * p.rows + row0 + r0) * p.cols + col;
 #pragma unroll
@@ -310,7 +312,12 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
         const int cb = now.cb;
         int t, row0, n;
         int64_t matrix;
-        place(now, t, matrix, row0, n);
+        if (RING && !(MODE & kWeight) && p.offsets) {
+            __syncwarp();
+            t = now.rest, matrix = 0, row0 = found[warp][stage].x, n = found[warp][stage].y;
+        } else {
+            place(now, t, matrix, row0, n);
+        }
         asm volatile("cp.async.wait_group %0;" ::"n"(D - 1) : "memory");
         P v;
         const int col = cb * 128 + c0;

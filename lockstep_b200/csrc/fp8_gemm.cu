@@ -34,7 +34,7 @@ constexpr int kBlock = 128;             // values of K per stage = per scale blo
 constexpr int kSegment = 32;            // blocks per accumulation chain of the LONG kernels
 enum Form { NT = 0, NN = 1, TN = 2 };
 
-constexpr int kStagingWords = 32 * 17;  // one epilogue warp's 32 rows x 16 columns, padded against bank conflicts
+constexpr int kStagingWords = 512;      // one epilogue warp's staging area: 16 rows of 128 bytes
 
 template <int CTAS, int BN>
 struct Fp8Cfg {
@@ -49,10 +49,11 @@ struct Fp8Cfg {
     static constexpr int ACC1 = BN - OVL;
     static constexpr int SFA_COL = 2 * BN - OVL, SFB_COL = SFA_COL + 4;
     static_assert(SFB_COL + 4 * SFB_TILES <= kTmemCols, "tensor memory overflow");
-    static constexpr int TAIL = STAGES * STAGE_BYTES;      // barriers, the groups' tile prefix, the epilogue warps' staging
+    static constexpr int STAGING = STAGES * STAGE_BYTES;   // of the epilogue warps; then barriers, the groups' tile prefix
+    static constexpr int TAIL = STAGING + 8 * kStagingWords * 4;
     static constexpr int LIST = TAIL + 256;
-    static constexpr int STAGING = LIST + 4 * (kFp8MaxGroups + 4);
-    static constexpr int SMEM = STAGING + 8 * kStagingWords * 4 + 1024;
+    static constexpr int SMEM = LIST + 4 * (kFp8MaxGroups + 4) + 1024;
+    static_assert(STAGING % 1024 == 0, "swizzled tiles start on 1024-byte boundaries");
     static_assert(SMEM <= 227 * 1024, "shared memory overflow");
 };
 
@@ -105,13 +106,26 @@ __device__ __forceinline__ void store_ragged(uint32_t *stage, int row_end, int N
     const int j = lane & 15, up = lane & 16;                       // rows i (lanes 0-15) and i + 16: different banks
     const int left = min(N - col0, 32), rows = row_end - row0 - up;
     const int64_t at = int64_t(row0 + up) * N + col0;
-    const uint32_t *from = stage + 17 * up + j;
+    if (lane == 0) ptx::bulk_wait_read();                          // a store_rows before has read the area
+    // Row k is 16 words at 16 k, its four 16-byte pieces permuted by (k / 2) % 4: eight lanes then write
+    // different banks, and reading row up + i the permutation is a constant of the unrolled loop.
+    uint4 *put = reinterpret_cast<uint4 *>(stage) + 4 * lane;
+    const int turn = (lane >> 1) & 3;
+    const uint32_t *from[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) from[c] = stage + 16 * up + (((j >> 2) ^ c) << 2) + (j & 3);
+    auto row = [&](int i) { return from[(i >> 1) & 3][16 * i]; };
     if (bf16) {
         __syncwarp();                                              // the staging area has been read
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-            stage[17 * lane + i] = *reinterpret_cast<const uint32_t *>(&h);
+        for (int c = 0; c < 4; c++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(r[8 * c + 2 * i]), __uint_as_float(r[8 * c + 2 * i + 1]));
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+            put[c ^ turn] = make_uint4(w[0], w[1], w[2], w[3]);
         }
         __syncwarp();
         uint16_t *dst = static_cast<uint16_t *>(cbase) + at + 2 * j;
@@ -119,16 +133,16 @@ __device__ __forceinline__ void store_ragged(uint32_t *stage, int row_end, int N
             const bool in = 2 * j < left;
 #pragma unroll
             for (int i = 0; i < 16; i++)
-                if (in && i < rows) *reinterpret_cast<uint32_t *>(dst + i * int64_t(N)) = from[17 * i];
+                if (in && i < rows) *reinterpret_cast<uint32_t *>(dst + i * int64_t(N)) = row(i);
             return;
         }
         // every other row starts on a pair (the same ones in both halves of the warp)
         if (row0 & 1) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) store_pair(dst + i * int64_t(N), from[17 * i], (i & 1) == 0, j, left, i < rows);
+            for (int i = 0; i < 16; i++) store_pair(dst + i * int64_t(N), row(i), (i & 1) == 0, j, left, i < rows);
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; i++) store_pair(dst + i * int64_t(N), from[17 * i], (i & 1) != 0, j, left, i < rows);
+            for (int i = 0; i < 16; i++) store_pair(dst + i * int64_t(N), row(i), (i & 1) != 0, j, left, i < rows);
         }
         return;
     }
@@ -137,13 +151,35 @@ __device__ __forceinline__ void store_ragged(uint32_t *stage, int row_end, int N
         if (16 * h >= left) return;
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 16; i++) stage[17 * lane + i] = r[16 * h + i];
+        for (int c = 0; c < 4; c++)
+            put[c ^ turn] = make_uint4(r[16 * h + 4 * c], r[16 * h + 4 * c + 1], r[16 * h + 4 * c + 2], r[16 * h + 4 * c + 3]);
         __syncwarp();
         uint32_t *dst = static_cast<uint32_t *>(cbase) + at + 16 * h + j;
         const bool in = 16 * h + j < left;
 #pragma unroll
         for (int i = 0; i < 16; i++)
-            if (in && i < rows) dst[i * int64_t(N)] = from[17 * i];
+            if (in && i < rows) dst[i * int64_t(N)] = row(i);
+    }
+}
+
+// Stores 32 rows of 128 bytes (64 bf16 or 32 fp32 columns; lane l holds row l as 32 words) by TMA through
+// the warp's staging area, 16 rows at a time: whole lines, and no address arithmetic or shuffles
+// per piece.  Columns past the tensor are clipped; the caller sees to it that all rows may be stored.
+__device__ __forceinline__ void store_rows(uint32_t stage, const CUtensorMap *map, int lane, int col0, int row0, int g, const uint32_t (&w)[32])
+{
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        if (lane == 0) ptx::bulk_wait_read();                      // the store before has read the area
+        __syncwarp();
+        if ((lane >> 4) == h) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                             ::"r"(stage + (lane & 15) * 128 + ((j ^ (lane & 7)) << 4)), "r"(w[4 * j]), "r"(w[4 * j + 1]), "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
+            ptx::fence_async_shared();
+        }
+        __syncwarp();
+        if (lane == 0) ptx::tma_store_3d(map, stage, col0, row0 + 16 * h, g);
     }
 }
 
@@ -165,7 +201,8 @@ struct Item {
 template <int CTAS, int BN, int FORM, bool LONG>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb, const Fp8Params p)
+                const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb,
+                const __grid_constant__ CUtensorMap tm_c, const Fp8Params p)
 {
     using C = Fp8Cfg<CTAS, BN>;
     constexpr bool A_MN = FORM == TN, B_MN = FORM != NT;
@@ -386,6 +423,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         const bool bf16 = p.out_bf16 != 0;
         uint32_t *stage = reinterpret_cast<uint32_t *>(gen_base + C::STAGING) + (warp - 2) * kStagingWords;
         const bool vec = p.N % (bf16 ? 8 : 4) == 0;
+        const uint32_t stage_addr = smem_base + C::STAGING + (warp - 2) * kStagingWords * 4;
         int lt = 0;
         bool ok = true;
         for (int t = worker; t < items && ok; t += workers) {
@@ -393,10 +431,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             constexpr int CH = BN / 64;                     // chunks of 32 columns per warp
             uint8_t *dst = static_cast<uint8_t *>(p.c) + (FORM == TN ? int64_t(it.g) * p.M * p.N * (bf16 ? 2 : 4) : 0);
             const int row = it.row0 + 32 * q;
+            const bool tma = BN >= 128 && vec && row + 32 <= it.row_end;           // uniform over the warp
+            const int zc = FORM == TN ? it.g : 0;
             auto emit = [&](int c, const uint32_t (&r)[32]) {
                 const int col0 = it.n0 + 32 * c;
-                if (vec && col0 + 32 <= p.N) store_chunk(it.row_end, p.N, dst, bf16, row, lane, col0, r);
-                else store_ragged(stage, it.row_end, p.N, dst, bf16, row, lane, col0, r);
+                if (!vec) store_ragged(stage, it.row_end, p.N, dst, bf16, row, lane, col0, r);
+                else if (!tma || bf16) store_chunk(it.row_end, p.N, dst, bf16, row, lane, col0, r);
+                else if (col0 < p.N) store_rows(stage_addr, &tm_c, lane, col0, row, zc, r);
             };
             if (it.nkb == 0) {
                 uint32_t z[32];
@@ -460,27 +501,62 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             ptx::tc_fence_after();
             const uint32_t acc = tmem_base + ((lt & 1) ? C::ACC1 : 0) + (uint32_t(32 * q) << 16);
             const bool owner = C::OVL > 0 && ((lt & 1) ? half == 0 : half == 1);
-            const int start = (owner && !(lt & 1)) ? CH - 1 : 0;
-            auto chunk = [&](int i) { return CH * half + (C::OVL > 0 ? ((start + i) & (CH - 1)) : i); };
             if (C::OVL > 0 && !owner) release();
-            uint32_t ra[32], rb[32];                        // the next chunk's load is in flight while this one is stored
-            ptx::tmem_ld32(acc + 32 * chunk(0), ra);
-#pragma unroll 1
-            for (int i = 0; i < CH; i += 2) {
+            uint32_t ra[32], rb[32];
+            if constexpr (CH == 1) {
+                ptx::tmem_ld32(acc + 32 * half, ra);
                 ptx::tmem_ld_wait(ra);
-                if (i + 1 < CH) ptx::tmem_ld32(acc + 32 * chunk(i + 1), rb);
-                else if (C::OVL == 0) release();
-                if (i == 0 && owner) release();
-                emit(chunk(i), ra);
-                if (i + 1 < CH) {
+                release();
+                emit(half, ra);
+            } else if (!vec) {
+                // chunk after chunk; the next one's load is in flight while this one is stored
+                const int start = owner && !(lt & 1) ? CH - 1 : 0;
+                auto chunk = [&](int i) { return CH * half + (C::OVL > 0 ? ((start + i) & (CH - 1)) : i); };
+                ptx::tmem_ld32(acc + 32 * chunk(0), ra);
+#pragma unroll 1
+                for (int i = 0; i < CH; i += 2) {
+                    ptx::tmem_ld_wait(ra);
+                    ptx::tmem_ld32(acc + 32 * chunk(i + 1), rb);
+                    if (i == 0 && owner) release();
+                    store_ragged(stage, it.row_end, p.N, dst, bf16, row, lane, it.n0 + 32 * chunk(i), ra);
                     ptx::tmem_ld_wait(rb);
                     if (i + 2 < CH) ptx::tmem_ld32(acc + 32 * chunk(i + 2), ra);
                     else if (C::OVL == 0) release();
-                    emit(chunk(i + 1), rb);
+                    store_ragged(stage, it.row_end, p.N, dst, bf16, row, lane, it.n0 + 32 * chunk(i + 1), rb);
+                }
+            } else {
+                // pairs of chunks (64 bf16 columns are whole lines), the one with the shared columns first
+                const int first = owner && !(lt & 1) ? CH / 2 - 1 : 0;
+#pragma unroll 1
+                for (int i = 0; i < CH / 2; i++) {
+                    const int c = CH * half + 2 * (first ^ i), col0 = it.n0 + 32 * c;
+                    ptx::tmem_ld32(acc + 32 * c, ra);
+                    ptx::tmem_ld32(acc + 32 * c + 32, rb);
+                    ptx::tmem_ld_wait(ra);
+                    ptx::tmem_ld_wait(rb);
+                    if (i == 0 && owner) release();
+                    if (C::OVL == 0 && i == CH / 2 - 1) release();
+                    if (!tma) {
+                        store_chunk(it.row_end, p.N, dst, bf16, row, lane, col0, ra);
+                        store_chunk(it.row_end, p.N, dst, bf16, row, lane, col0 + 32, rb);
+                    } else if (!bf16) {
+                        if (col0 < p.N) store_rows(stage_addr, &tm_c, lane, col0, row, zc, ra);
+                        if (col0 + 32 < p.N) store_rows(stage_addr, &tm_c, lane, col0 + 32, row, zc, rb);
+                    } else if (col0 < p.N) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int k = 0; k < 16; k++) {
+                            const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(ra[2 * k]), __uint_as_float(ra[2 * k + 1]));
+                            const __nv_bfloat162 y = __floats2bfloat162_rn(__uint_as_float(rb[2 * k]), __uint_as_float(rb[2 * k + 1]));
+                            w[k] = *reinterpret_cast<const uint32_t *>(&x), w[16 + k] = *reinterpret_cast<const uint32_t *>(&y);
+                        }
+                        store_rows(stage_addr, &tm_c, lane, col0, row, zc, w);
+                    }
                 }
             }
             lt++;
         }
+        if (lane == 0) ptx::bulk_wait_all();                // (none of its own: returns at once)
         if (FORM != TN && p.offsets && p.zero_tail) {       // rows behind the last group
             const int64_t bytes = int64_t(p.N) * (bf16 ? 2 : 4);
             uint8_t *dst = static_cast<uint8_t *>(p.c);
@@ -512,14 +588,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 // ---- host ---------------------------------------------------------------------
 struct MapSpec {
     const void *base;
-    int64_t inner, rows, depth;    // bytes (u8) or words (scales), rows, matrices
+    int64_t inner, rows, depth;    // elements, rows, matrices
     int64_t pitch;                 // bytes between rows
     int box_inner, box_rows;
-    bool scales;
+    MapType type;
     bool operator==(const MapSpec &o) const
     {
         return base == o.base && inner == o.inner && rows == o.rows && depth == o.depth && pitch == o.pitch &&
-               box_inner == o.box_inner && box_rows == o.box_rows && scales == o.scales;
+               box_inner == o.box_inner && box_rows == o.box_rows && type == o.type;
     }
 };
 
@@ -530,11 +606,11 @@ int make_map(CUtensorMap *m, const MapSpec &k)
     struct Slot { MapSpec key; CUtensorMap map; bool used; };
     static thread_local Slot slots[256] = {};
     uint64_t h = (reinterpret_cast<uintptr_t>(k.base) >> 4) ^ uint64_t(k.rows) * 0x9E3779B97F4A7C15ull ^
-                 uint64_t(k.inner) * 0xC2B2AE3D27D4EB4Full ^ uint64_t(k.depth * 131 + k.pitch * 31 + k.box_rows * 7 + k.scales);
+                 uint64_t(k.inner) * 0xC2B2AE3D27D4EB4Full ^ uint64_t(k.depth * 131 + k.pitch * 31 + k.box_rows * 7 + k.type);
     h ^= h >> 29;
     Slot &slot = slots[h % 256];
     if (!slot.used || !(slot.key == k)) {
-        if (int rc = encode_map_3d(&slot.map, k.base, k.inner, k.rows, k.depth, k.pitch, k.box_inner, k.box_rows, k.scales)) {
+        if (int rc = encode_map_3d(&slot.map, k.base, k.inner, k.rows, k.depth, k.pitch, k.box_inner, k.box_rows, k.type)) {
             slot.used = false;
             return rc;
         }
@@ -545,7 +621,7 @@ int make_map(CUtensorMap *m, const MapSpec &k)
 }
 
 template <int CTAS, int BN, int FORM, bool LONG>
-int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa, const CUtensorMap &tsb, const Fp8Params &p,
+int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa, const CUtensorMap &tsb, const CUtensorMap &tc, const Fp8Params &p,
            int64_t most_tiles, cudaStream_t st)
 {
     using C = Fp8Cfg<CTAS, BN>;
@@ -577,7 +653,7 @@ int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa,
     lk.unlock();
     cfg.gridDim = dim3(unsigned(CTAS * workers), 1, 1);
     cfg.attrs = at, cfg.numAttrs = CTAS == 2 ? 2 : 1;
-    LS_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<CTAS, BN, FORM, LONG>, ta, tb, tsa, tsb, p));
+    LS_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<CTAS, BN, FORM, LONG>, ta, tb, tsa, tsb, tc, p));
     return LS_OK;
 }
 
@@ -666,13 +742,18 @@ int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t 
     if (form != TN)
         for (a_box = 16; a_box < M && a_box < 128; a_box *= 2) {}
     p.a_bytes = a_box * kBlock;
-    if (int rc = make_map(&ta, {a, a_extent, a_rows, 1, lda, 128, a_box, false})) return rc;
-    if (int rc = make_map(&tb, {b, b_extent, b_rows, depth, ldb, 128, form == NT && bn == 64 ? 64 : 128, false})) return rc;
-    if (int rc = make_map(&tsa, {sfa, 128, a_tiles, 1, 512, 128, 1, true})) return rc;
-    if (int rc = make_map(&tsb, {sfb, 128, b_tiles, 1, 512, 128, 1, true})) return rc;
+    if (int rc = make_map(&ta, {a, a_extent, a_rows, 1, lda, 128, a_box, kMapBytes})) return rc;
+    if (int rc = make_map(&tb, {b, b_extent, b_rows, depth, ldb, 128, form == NT && bn == 64 ? 64 : 128, kMapBytes})) return rc;
+    if (int rc = make_map(&tsa, {sfa, 128, a_tiles, 1, 512, 128, 1, kMapWords})) return rc;
+    if (int rc = make_map(&tsb, {sfb, 128, b_tiles, 1, 512, 128, 1, kMapWords})) return rc;
+    // C, stored in boxes of 16 rows x 128 bytes; rows that do not start on 16-byte boundaries have no map
+    CUtensorMap tc = ta;
+    const int64_t es = p.out_bf16 ? 2 : 4;
+    if (N * es % 16 == 0)
+        if (int rc = make_map(&tc, {c, N, M, form == TN ? groups : 1, N * es, int(128 / es), 16, p.out_bf16 ? kMapBf16 : kMapF32})) return rc;
     const bool many = out_dtype == LS_F32 && kblocks > kSegment;
 #define LS_FP8_LAUNCH(C, B, F) \
-    return many ? launch<C, B, F, true>(ta, tb, tsa, tsb, p, items, st) : launch<C, B, F, false>(ta, tb, tsa, tsb, p, items, st)
+    return many ? launch<C, B, F, true>(ta, tb, tsa, tsb, tc, p, items, st) : launch<C, B, F, false>(ta, tb, tsa, tsb, tc, p, items, st)
 #define LS_FP8_FORM(F)                          \
     if (form == F) {                            \
         if (pair) LS_FP8_LAUNCH(2, 256, F);     \

@@ -947,7 +947,7 @@ void splitk_release(cudaStream_t st)
 }  // namespace
 
 int encode_map_3d(void *map, const void *base, int64_t inner, int64_t rows, int64_t depth, int64_t pitch, int box_inner,
-                  int box_rows, bool words)
+                  int box_rows, MapType type)
 {
     EncodeFn fn = encode_fn();
     if (!fn) return fail(LS_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
@@ -955,9 +955,11 @@ int encode_map_3d(void *map, const void *base, int64_t inner, int64_t rows, int6
     cuuint64_t strides[2] = {cuuint64_t(pitch), cuuint64_t(pitch) * cuuint64_t(rows)};
     cuuint32_t box[3] = {cuuint32_t(box_inner), cuuint32_t(box_rows), 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = fn(static_cast<CUtensorMap *>(map), words ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3,
-                    const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    words ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const CUtensorMapDataType types[] = {CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                         CU_TENSOR_MAP_DATA_TYPE_FLOAT32};
+    CUresult r = fn(static_cast<CUtensorMap *>(map), types[type], 3, const_cast<void *>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    type == kMapWords ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(LS_ECUDA, "cuTensorMapEncodeTiled failed with %d", int(r));
     return LS_OK;
