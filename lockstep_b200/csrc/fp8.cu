@@ -185,15 +185,15 @@ fp8_rows_kernel(const T *__restrict__ x, int64_t rows, int K, const int *__restr
 // kRows: blocks along the rows; kCols: blocks down the columns (kRows | kCols from one read);
 // kWeight: one block for the whole tile, its scale to both scale layouts.
 //
-// Persistent CTAs of 512 threads, two per SM; a thread owns 8 columns of 4 rows of a tile: lane l of
-// warp w has columns 8 (l % 16) .. + 7 of rows 8 w + l / 16 + 2 i.  bf16: each thread copies its own
-// 16-byte pieces of the next tiles to shared memory ahead of time (cp.async, waited for by itself:
-// the ring needs no barrier), so loads stay in flight while a tile is reduced; holding tiles in
-// registers without the ring left one CTA of 256 threads per SM and took 205 us for 16384 x 4096
-// in both forms.  fp32 tiles are loaded straight to registers (a ring of them leaves room for one CTA
-// per SM: 99 us against 61 for 8192 x 8192 weights).
-// bf16 magnitudes are compared two at a time as 16-bit integers.  Non-finite values (rare) are set
-// to zero for the maxima and patched into the codes afterwards.
+// Persistent CTAs; a thread owns 8 columns of R rows of a tile (bf16: 8 rows, 256 threads, three CTAs per
+// SM; fp32: 4 rows, 512 threads, two): lane l of warp w has columns 8 (l % 16) .. + 7 of rows
+// 2 R w + l / 16 + 2 i.  bf16: each thread copies its own 16-byte pieces of the next tiles to shared
+// memory ahead of time (cp.async, waited for by itself: the ring needs no barrier), so loads stay in
+// flight while a tile is reduced.  16384 x 4096 in both forms: 51.4 us = 5.2 TB/s (205 us with the tile in
+// registers and no ring, 52.7 with 4 rows per thread); bound by issue slots, three quarters of them
+// used.  fp32 tiles are loaded straight to registers (a ring of them leaves room for one CTA per SM:
+// 99 us against 55 for 8192 x 8192 weights).
+// Non-finite values (rare) are set to zero for the maxima and patched into the codes afterwards.
 enum { kRows = 1, kCols = 2, kWeight = 4 };
 
 struct TileArgs {
@@ -210,20 +210,20 @@ struct TileArgs {
     uint8_t *sf_t;                  // rows = columns of x, blocks = row slots
 };
 
-// A thread's 4 x 8 values: bf16 as 4 words per row, fp32 as 8.
+// A thread's R x 8 values: bf16 as 4 words per row, fp32 as 8.
 template <typename T> struct Piece {
     using W = Word<T>;
     static constexpr int WORDS = sizeof(T) == 2 ? 4 : 8, CHUNKS = WORDS / 4;
-    static constexpr int R = 4, THREADS = 2048 / R;
+    static constexpr int R = sizeof(T) == 2 ? 8 : 4, THREADS = 2048 / R;
     uint32_t u[R][WORDS];
     // sets non-finite values to zero; bit 8 i + j: value (i, j) was one
-    __device__ __forceinline__ uint32_t drop_special()
+    __device__ __forceinline__ uint64_t drop_special()
     {
-        uint32_t flags = 0;
+        uint64_t flags = 0;
 #pragma unroll
         for (int i = 0; i < R; i++)
 #pragma unroll
-            for (int w = 0; w < WORDS; w++) flags |= W::drop_special(u[i][w]) << (8 * i + 8 / WORDS * w);
+            for (int w = 0; w < WORDS; w++) flags |= uint64_t(W::drop_special(u[i][w])) << (8 * i + 8 / WORDS * w);
         return flags;
     }
     // fp32 bits of the largest magnitude of row i
@@ -244,11 +244,11 @@ template <typename T> struct Piece {
     }
 };
 
-constexpr int kRing = 3;                                    // tiles of the ring: 96 KB, two CTAs per SM
+constexpr int kRing = 2;                                    // tiles of the ring: 64 KB, three CTAs per SM
 constexpr int kRingBytes = kRing * 128 * 128 * 2;
 
 template <typename T, bool VEC, int MODE>
-__global__ void __launch_bounds__(Piece<T>::THREADS, 2)
+__global__ void __launch_bounds__(Piece<T>::THREADS, sizeof(T) == 2 ? 3 : 2)
 fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
 {
     begin_dependent_launch();
@@ -348,7 +348,7 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
         }
         stage = stage + 1 == D ? 0 : stage + 1;
         if (n <= 0) continue;                               // a slot without rows; uniform over the CTA
-        uint32_t flags = 0;
+        uint64_t flags = 0;
         const bool special = __any_sync(0xFFFFFFFFu, most >= kBitsInf);
         if (special) {
             flags = v.drop_special();
@@ -358,7 +358,7 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
         }
         auto put = [&](uint8_t *dst, int i, const uint32_t (&inv)[P::WORDS]) {
             *reinterpret_cast<uint2 *>(dst) = make_uint2(W::codes(v.u[i], inv), W::codes(v.u[i] + P::WORDS / 2, inv + P::WORDS / 2));
-            if (special) store_nans(dst, (flags >> (8 * i)) & 0xFFu);
+            if (special) store_nans(dst, uint32_t(flags >> (8 * i)) & 0xFFu);
         };
         auto put_all = [&](uint8_t *dst, int i, uint32_t s) {      // one scale for the row's values
             uint32_t inv[P::WORDS];
@@ -395,17 +395,23 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
             }
         }
         if constexpr (MODE & kRows) {
-            // Maxima of the 4 rows over 16 lanes: two exchanges that halve what a lane keeps (its row is
-            // then the upper two of its four lane bits), two plain steps, and the scales sent back:
-            // 9 shuffles instead of 16.
-            const bool b3 = lane & 8, b2 = lane & 4;
-            const uint32_t x0 = __shfl_xor_sync(0xFFFFFFFFu, b3 ? m[0] : m[2], 8), x1 = __shfl_xor_sync(0xFFFFFFFFu, b3 ? m[1] : m[3], 8);
-            const uint32_t y0 = max(b3 ? m[2] : m[0], x0), y1 = max(b3 ? m[3] : m[1], x1);
-            uint32_t z = max(b2 ? y1 : y0, __shfl_xor_sync(0xFFFFFFFFu, b2 ? y0 : y1, 4));
-            z = max(z, __shfl_xor_sync(0xFFFFFFFFu, z, 2));
-            z = max(z, __shfl_xor_sync(0xFFFFFFFFu, z, 1));
-            const uint32_t e8 = fp8_e8m0(z);
+            // Maxima of the R rows over 16 lanes: exchanges that halve what a lane keeps (its row is then the
+            // upper log2 R of its four lane bits), plain steps for the other bits, and the scales
+            // sent back: 16 shuffles instead of 32 for eight rows.
             constexpr int SHARE = 16 / R;                   // lanes that end up with the same row
+#pragma unroll
+            for (int h = R / 2, o = 8; h > 0; h /= 2, o /= 2) {
+                const bool up = lane & o;
+#pragma unroll
+                for (int k = 0; k < h; k++) {
+                    const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, up ? m[k] : m[k + h], o);
+                    m[k] = max(up ? m[k + h] : m[k], got);
+                }
+            }
+            uint32_t z = m[0];
+#pragma unroll
+            for (int o = SHARE / 2; o > 0; o /= 2) z = max(z, __shfl_xor_sync(0xFFFFFFFFu, z, o));
+            const uint32_t e8 = fp8_e8m0(z);
             const int mine = r0 + 2 * ((lane & 15) / SHARE);
             if (lane % SHARE == 0 && mine < n) p.sf[sf_offset(uint32_t(128 * t + mine), uint32_t(cb), uint32_t(kt))] = uint8_t(e8);
 #pragma unroll
@@ -501,7 +507,7 @@ int launch_tile_kernel(const void *x, const TileArgs &p, int64_t tiles, cudaStre
             attr_set[dev] = true;
         }
     }
-    const int64_t most = int64_t(sm_count()) * 2;
+    const int64_t most = int64_t(sm_count()) * (sizeof(T) == 2 ? 3 : 2);
     return launch_dependent(fp8_tile_kernel<T, VEC, MODE>, dim3(unsigned(std::min(tiles, most))), Piece<T>::THREADS, ring, st,
                             static_cast<const T *>(x), p);
 }

@@ -76,9 +76,9 @@ __device__ __forceinline__ uint32_t cvt_e4m3x4(float a, float b, float c, float 
 constexpr uint32_t kAbs = 0x7FFFFFFFu;
 
 // Values are kept as the 32-bit words they were loaded in: one fp32 value, or two bf16 values.
-// bf16 pairs are handled two at a time: packed NaN-propagating maxima of magnitudes (a 16-bit
-// integer maximum of pairs is several instructions), and scaled by a packed multiplication, which is
-// exact (a power of two; results below bf16's range are far below E4M3's).
+// bf16 pairs are handled two at a time: NaN-propagating maxima of magnitudes that need no masking of
+// signs, and a packed multiplication by the reciprocal scale, which is exact (a power of two; results
+// below bf16's range are far below E4M3's).
 template <typename T> struct Word {
     static constexpr bool PAIR = sizeof(T) == 2;
     // the larger magnitude (per half), NaN if either is one; the result's sign means nothing
