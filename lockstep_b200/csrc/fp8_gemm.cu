@@ -266,7 +266,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                 list_pre[g] = before + sum - own;
                 if (g == p.groups - 1) list_pre[p.groups] = before + sum;
             }
-            before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+            before = min(before + __shfl_sync(0xFFFFFFFFu, sum, 31), 1 << 30);     // (only offsets out of order reach the limit)
         }
     }
     ptx::tc_fence_before();
@@ -276,7 +276,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     const uint32_t tmem_base = *tmem_slot_p;
 
     // ---- the list of tiles, the same for every role
-    const int m_tiles = FORM == TN || !p.offsets ? (p.M + 128 * CTAS - 1) / (128 * CTAS) : list_pre[p.groups];
+    // (more tiles than ordered offsets can have would be those of overlapping groups: no sense, and no bound)
+    const int m_tiles = FORM == TN || !p.offsets ? (p.M + 128 * CTAS - 1) / (128 * CTAS)
+                                                 : min(list_pre[p.groups], p.M / (128 * CTAS) + p.groups);
     const int n_tiles = (p.N + BN - 1) / BN;
     const int items = m_tiles * n_tiles * (FORM == TN ? p.groups : 1);
     auto item_of = [&](int t) {
@@ -299,9 +301,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             int lo = 0, hi = p.M, i = t, mine = m_tiles;
             if (p.offsets) {
                 int a = 0, b = p.groups - 1;                // last group whose tiles start at or before t
+                const int column = t / n_tiles;
                 while (a < b) {
                     const int m = (a + b + 1) >> 1;
-                    if (list_pre[m] * n_tiles <= t) a = m;
+                    if (list_pre[m] <= column) a = m;
                     else b = m - 1;
                 }
                 it.g = a;
@@ -673,6 +676,7 @@ int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t 
     if (!c) return fail(LS_EINVAL, "null pointer");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (K == 0) {                                           // empty sums
+        if (offsets && form != TN && !zero_tail) return fail(LS_EINVAL, "K must be positive where rows of no group are kept");
         LS_CUDA(cudaMemsetAsync(c, 0, size_t(form == TN ? groups : 1) * M * N * (out_dtype == LS_BF16 ? 2 : 4), st));
         return LS_OK;
     }

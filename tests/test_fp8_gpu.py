@@ -172,6 +172,25 @@ def test_weight_gradient_product(M, N, K, variant):
     _close(c, *ref.grad_weight(gy, x), f"TN {M}x{N}x{K}")
 
 
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(5000, 2040, 300), (4600, 2041, 260), (260, 9000, 5000)])
+def test_many_tiles_per_cta(M, N, K, out, variant):
+    # several tiles, and for fp32 several accumulation chains, pass through every accumulator of a CTA
+    from lockstep_b200 import fp8
+    x, w = _data(M, K, seed=1), _data(N, K, seed=2)
+    xc, xsf = fp8.quantize_fp8_packed(x)
+    wc, wsf, _ = fp8.quantize_fp8_weight(w)
+    _close(fp8.fp8_gemm(xc, wc, xsf, wsf, out), *ref.forward(x, w), f"NT {M}x{N}x{K}")
+    w = _data(K, N, seed=3)
+    wc, _, wsf_t = fp8.quantize_fp8_weight(w)
+    _close(fp8.fp8_gemm_nn(xc, wc, xsf, wsf_t, out), *ref.grad_input(x, w), f"NN {M}x{N}x{K}")
+    gy, v = _data(K, M, seed=4), _data(K, N, seed=5)
+    _, _, gct, gsf_t = fp8.quantize_fp8_both(gy)
+    _, _, vct, vsf_t = fp8.quantize_fp8_both(v)
+    _close(fp8.fp8_gemm_tn(gct, vct, gsf_t, vsf_t, out), *ref.grad_weight(gy, v), f"TN {M}x{N}x{K}")
+    _status()
+
+
 def test_long_sums_are_as_exact_as_short_ones(variant):
     # fp32 output: the K loop is cut into chains of 4096 values, each with an error e relative to its sum;
     # the sum of m of them has at most m e |chain| ~ sqrt(m) e |sum| if all errors point one way.  (One
@@ -197,11 +216,37 @@ def test_long_sums_are_as_exact_as_short_ones(variant):
 
 
 # ---------------------------------------------------------------- grouped
+MANY = [0, 1, 3, 130, 0, 0, 2, 40] * 128                      # 1024 groups
 GROUPS = [[128], [0], [5, 0, 0, 300, 1, 0], [128, 128, 256], [1] * 40, [129, 127, 2, 640, 0, 33], [0, 0, 7], [1000, 3]]
 
 
 def _offsets(sizes, dtype=torch.int32):
     return torch.tensor(np.concatenate([[0], np.cumsum(sizes)]), dtype=dtype, device="cuda")
+
+
+def test_as_many_groups_as_there_may_be():
+    from lockstep_b200 import fp8, fp8_linear
+    G, T, K, N = len(MANY), sum(MANY) + 5, 128, 72
+    x, gy, w = _data(T, K, seed=7), _data(T, N, seed=8), _data(G, N, K, seed=9)
+    off = _offsets(MANY)
+    xi, wi = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = fp8_linear.grouped_linear(xi, wi, off)
+    y.backward(gy)
+    codes, sf, _ = fp8.quantize_fp8_weight(w)
+    assert torch.equal(fp8_linear.grouped_linear_quantized(x, codes, sf, off), y)
+    _status()
+    bounds = off.tolist()
+    for g in list(range(0, 24)) + list(range(1000, 1024)):
+        r = slice(bounds[g], bounds[g + 1])
+        if bounds[g] == bounds[g + 1]:
+            assert (wi.grad[g] == 0).all()
+            continue
+        _close(y.detach()[r], *ref.forward(x[r], w[g]), f"y of group {g}")
+        _close(xi.grad[r], *ref.grad_input(gy[r], w[g]), f"gx of group {g}")
+        _close(wi.grad[g], *ref.grad_weight(gy[r], x[r]), f"gw of group {g}")
+    assert (y[bounds[-1]:] == 0).all() and (xi.grad[bounds[-1]:] == 0).all()
+    few = fp8_linear.grouped_linear_quantized(x[:20], codes, sf, off.clamp_max(20))
+    _close(few[1:4], *ref.forward(x[1:4], w[2]), "group 2 of a few rows")
 
 
 @pytest.mark.parametrize("N,K", [(128, 128), (264, 1000), (513, 200)])
@@ -401,6 +446,7 @@ def test_abi_refusals():
     assert serve(rows=2, x=None) == serve(rows=2, ldw=100) == serve(rows=2, w=None) == EINVAL and serve(rows=2, w=odd) == EALIGN
     assert L.ls_fp8_linear_forward(p, 0, p, 0, 4, 4, 128, None, 1, 3, p, None, p, stream()) == EINVAL       # nowhere to keep
     assert L.ls_fp8_linear_forward(p, 0, p, 0, 4, 4, 128, None, 1, 4, p, p, p, stream()) == EINVAL
+    assert L.ls_fp8_gemm_grouped(0, p, 128, p, 128, p, p, p, 0, 4, 4, 0, ptr(off), 1, 0, stream()) == EINVAL
     assert L.ls_fp8_gemm_set_variant(5) == EINVAL
     torch.cuda.synchronize()
 
