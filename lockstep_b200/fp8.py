@@ -65,7 +65,7 @@ def slots(rows: int, groups: int) -> int:
 
 def _input(x, dims=2):
     if x.dim() != dims:
-        raise ValueError(f"expected a {dims}-dimensional tensor, got shape {tuple(x.shape)}")
+        raise AssertionError(f"expected a {dims}-dimensional tensor, got shape {tuple(x.shape)}")
     if x.dtype not in _DTYPE:
         x = x.float()
     return _aligned(x)
@@ -114,7 +114,7 @@ def _groups(offsets):
     if offsets is None:
         return None, 0
     if offsets.dim() != 1 or not 2 <= offsets.shape[0] <= MAX_GROUPS + 1:
-        raise ValueError(f"offsets: groups + 1 values, 1 to {MAX_GROUPS} groups; got shape {tuple(offsets.shape)}")
+        raise AssertionError(f"offsets: groups + 1 values, 1 to {MAX_GROUPS} groups; got shape {tuple(offsets.shape)}")
     if offsets.dtype != torch.int32:
         if offsets.dtype != torch.int64:
             raise TypeError(f"offsets must be int32 or int64, got {offsets.dtype}")
@@ -150,7 +150,7 @@ def quantize_fp8_packed(x: torch.Tensor, offsets: torch.Tensor = None):
     """x [..., K] -> (codes, sf): what the products take as their row operand.  With offsets
     (x two-dimensional), the codes keep x's row order and sf is in slot order."""
     if offsets is not None and x.dim() != 2:
-        raise ValueError("a grouped tensor is two-dimensional")
+        raise AssertionError("a grouped tensor is two-dimensional")
     codes, _, sf = _quantize_rows(x, offsets, False, True)
     return codes, sf
 
@@ -183,7 +183,7 @@ def quantize_fp8_weight(w: torch.Tensor, want_scale: bool = False):
         *lead, N, K = w.shape
         G, dev = lead[0] if lead else 1, w.device
         if G > MAX_GROUPS:
-            raise ValueError(f"at most {MAX_GROUPS} matrices, got {G}")
+            raise AssertionError(f"at most {MAX_GROUPS} matrices, got {G}")
         codes = _codes(lead, N, K, dev)
         sf, sf_t = _bytes((*lead, sf_bytes(N, K)), dev), _bytes((*lead, sf_bytes(K, N)), dev)
         scale = torch.empty((*lead, -(-N // BLOCK), -(-K // BLOCK)), dtype=torch.float32, device=dev) if want_scale else None
@@ -200,7 +200,7 @@ def dequantize_fp8(codes: torch.Tensor, scale: torch.Tensor, out_dtype=torch.flo
         kb = -(-K // BLOCK)
         row_block = 1 if scale.shape == (*codes.shape[:-1], kb) else BLOCK
         if row_block == BLOCK and scale.shape != (*lead, -(-rows // BLOCK), kb):
-            raise ValueError(f"scale shape {tuple(scale.shape)} does not fit codes {tuple(codes.shape)}")
+            raise AssertionError(f"scale shape {tuple(scale.shape)} does not fit codes {tuple(codes.shape)}")
         out = torch.empty(codes.shape, dtype=out_dtype, device=codes.device)
         scale = _aligned(scale.float())
 
@@ -238,20 +238,20 @@ _NT, _NN, _TN = 0, 1, 2
 
 def _sf(sf, want, what):
     if sf.dtype != torch.uint8 or sf.numel() != want:
-        raise ValueError(f"{what}: a scale-factor buffer of {want} bytes is needed, got {sf.numel()} of {sf.dtype}")
+        raise AssertionError(f"{what}: a scale-factor buffer of {want} bytes is needed, got {sf.numel()} of {sf.dtype}")
     return _aligned(sf)
 
 
 def _given(out, shape, dtype):
     if out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 16:
-        raise ValueError(f"out must be a contiguous, 16-byte aligned {tuple(shape)} tensor of {dtype}")
+        raise AssertionError(f"out must be a contiguous, 16-byte aligned {tuple(shape)} tensor of {dtype}")
     return out
 
 
 def _product(form, a, b, a_sf, b_sf, out_dtype, out, offsets, rows):
     with on_device_of(a, b, a_sf, b_sf, offsets, out):
         if a.dim() != 2 or b.dim() != (2 if offsets is None or form == _TN else 3):
-            raise ValueError(f"operand shapes {tuple(a.shape)} and {tuple(b.shape)}")
+            raise AssertionError(f"operand shapes {tuple(a.shape)} and {tuple(b.shape)}")
         off, G = _groups(offsets) if offsets is not None else (None, 1)
         if form == _TN:
             held, M = a.shape
@@ -259,7 +259,7 @@ def _product(form, a, b, a_sf, b_sf, out_dtype, out, offsets, rows):
             K = held if off is None else rows
             tiles = -(-held // BLOCK) * BLOCK if off is None else BLOCK * slots(K, G)
             if b.shape[0] != held or (off is not None and held != tiles):
-                raise ValueError(f"operands with {a.shape[0]} and {b.shape[0]} rows"
+                raise AssertionError(f"operands with {a.shape[0]} and {b.shape[0]} rows"
                                  + ("" if off is None else f", {tiles} needed for {K} rows in {G} groups"))
             a_sf, b_sf = _sf(a_sf, sf_bytes(M, tiles), "a_sf"), _sf(b_sf, sf_bytes(N, tiles), "b_sf")
             shape = (M, N) if off is None else (G, M, N)
@@ -267,7 +267,7 @@ def _product(form, a, b, a_sf, b_sf, out_dtype, out, offsets, rows):
             M, K = a.shape
             N, Kb = b.shape[-2:] if form == _NT else b.shape[-1:-3:-1]
             if Kb != K or (off is not None and b.shape[0] != G):
-                raise ValueError(f"operand shapes {tuple(a.shape)} and {tuple(b.shape)} do not fit" + ("" if off is None else f" {G} groups"))
+                raise AssertionError(f"operand shapes {tuple(a.shape)} and {tuple(b.shape)} do not fit" + ("" if off is None else f" {G} groups"))
             a_sf = _sf(a_sf, sf_bytes(M if off is None else BLOCK * slots(M, G), K), "a_sf")
             b_sf = _sf(b_sf, G * sf_bytes(N, K), "b_sf")
             shape = (M, N)

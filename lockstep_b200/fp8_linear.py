@@ -28,9 +28,9 @@ _GRAD_X, _GRAD_W = 1, 2
 
 def _check(x, w, dims):
     if w.dim() != dims:
-        raise ValueError(f"weight must be {dims}-dimensional, got shape {tuple(w.shape)}")
+        raise AssertionError(f"weight must be {dims}-dimensional, got shape {tuple(w.shape)}")
     if x.shape[-1] != w.shape[-1]:
-        raise ValueError(f"input of width {x.shape[-1]} for a weight of shape {tuple(w.shape)}")
+        raise AssertionError(f"input of width {x.shape[-1]} for a weight of shape {tuple(w.shape)}")
     if x.dtype not in fp8._DTYPE:
         raise TypeError(f"unsupported dtype {x.dtype}")
 
@@ -53,7 +53,7 @@ class _FP8Matmul(torch.autograd.Function):
         with on_device_of(x, w, offsets):
             off, G = fp8._groups(offsets)
             if off is not None and w.shape[0] != G:
-                raise ValueError(f"{w.shape[0]} experts for offsets of {G} groups")
+                raise AssertionError(f"{w.shape[0]} experts for offsets of {G} groups")
             xi, wi = fp8._aligned(x), fp8._input(w, w.dim())
             (rows, K), N, dev = xi.shape, w.shape[-2], x.device
             grads = (_GRAD_X if ctx.needs_input_grad[0] else 0) | (_GRAD_W if ctx.needs_input_grad[1] else 0)
@@ -96,9 +96,9 @@ def grouped_linear(x, weight, offsets):
     gradients.  Rows of no expert give zeros, also in their gradient."""
     _check(x, weight, 3)
     if x.dim() != 2:
-        raise ValueError(f"rows sorted by expert are two-dimensional, got shape {tuple(x.shape)}")
+        raise AssertionError(f"rows sorted by expert are two-dimensional, got shape {tuple(x.shape)}")
     if offsets is None:
-        raise ValueError("offsets are needed")
+        raise AssertionError("offsets are needed")
     return _FP8Matmul.apply(x, weight, offsets)
 
 
@@ -108,7 +108,7 @@ def _serve(x, codes, sf, offsets, out_dtype, out):
     with on_device_of(x, codes, sf, offsets, out):
         off, G = (None, 0) if offsets is None else fp8._groups(offsets)
         if off is not None and codes.shape[0] != G:
-            raise ValueError(f"{codes.shape[0]} experts for offsets of {G} groups")
+            raise AssertionError(f"{codes.shape[0]} experts for offsets of {G} groups")
         if not x.is_contiguous() or x.data_ptr() % 32:
             x = fp8._aligned(x)
         rows, K = x.shape
@@ -138,9 +138,9 @@ def grouped_linear_quantized(x, codes, sf, offsets, out_dtype=None, out=None):
     expert are left as they were."""
     _check(x, codes, 3)
     if x.dim() != 2:
-        raise ValueError(f"rows sorted by expert are two-dimensional, got shape {tuple(x.shape)}")
+        raise AssertionError(f"rows sorted by expert are two-dimensional, got shape {tuple(x.shape)}")
     if offsets is None:
-        raise ValueError("offsets are needed")
+        raise AssertionError("offsets are needed")
     return _serve(x, codes, sf, offsets, out_dtype, out)
 
 
