@@ -19,11 +19,18 @@ __device__ __noinline__ void store_nans(uint8_t *dst, uint32_t flags)
     for (; flags; flags &= flags - 1) dst[__ffs(flags) - 1] = 0x7F;
 }
 
-// 32 bytes in one instruction: two 16-byte loads of a lane would fetch every 32-byte sector twice
-__device__ __forceinline__ void ld_stream32(const void *p, uint32_t *w)
+// 32 bytes in one instruction: two 16-byte loads of a lane would fetch every 32-byte sector twice.
+// once: the tensor is too large to stay in L2 and its lines are the first to leave (33.2 -> 32.4 us for
+// 16384 x 4096 bf16 rows; a small tensor is read 0.2 us faster without, and in the tiles of both forms
+// below the same hint costs 5 %).
+__device__ __forceinline__ void ld_stream32(const void *p, uint32_t *w, bool once)
 {
-    asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+    if (once)
+        asm volatile("ld.global.nc.L1::no_allocate.L2::evict_first.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
+    else
+        asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7]) : "l"(p));
 }
 
 // ---- ragged groups ------------------------------------------------------------------------
@@ -67,7 +74,7 @@ __device__ __forceinline__ void slot_rows(const int *bounds, int groups, int t, 
 template <typename T> constexpr int kTurn = 32 * (16 + 16 / int(sizeof(T)));
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_chunk(const T *row, int chunk, int K, T *turn, uint32_t (&w)[8 * sizeof(T) / 2])
+__device__ __forceinline__ void load_chunk(const T *row, int chunk, int K, T *turn, bool once, uint32_t (&w)[8 * sizeof(T) / 2])
 {
     constexpr int WORDS = 8 * sizeof(T) / 2;
     const int lane = threadIdx.x & 31;
@@ -75,7 +82,7 @@ __device__ __forceinline__ void load_chunk(const T *row, int chunk, int K, T *tu
         const int col = chunk * 512 + lane * 16;
 #pragma unroll
         for (int h = 0; h < WORDS / 8; h++) {
-            if (col < K) ld_stream32(row + col + 32 / int(sizeof(T)) * h, w + 8 * h);
+            if (col < K) ld_stream32(row + col + 32 / int(sizeof(T)) * h, w + 8 * h, once);
             else
                 for (int i = 0; i < 8; i++) w[8 * h + i] = 0u;
         }
@@ -143,7 +150,7 @@ __device__ __forceinline__ void quantize_chunk(uint32_t (&w)[8 * sizeof(T) / 2],
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256, 4)
 fp8_rows_kernel(const T *__restrict__ x, int64_t rows, int K, const int *__restrict__ offsets, int groups,
-                uint8_t *__restrict__ codes, int64_t ld, float *__restrict__ scale, uint8_t *__restrict__ sf)
+                uint8_t *__restrict__ codes, int64_t ld, float *__restrict__ scale, uint8_t *__restrict__ sf, bool once)
 {
     begin_dependent_launch();
     __shared__ int bounds[kFp8MaxGroups + 1];
@@ -166,11 +173,11 @@ fp8_rows_kernel(const T *__restrict__ x, int64_t rows, int K, const int *__restr
         uint32_t a[8 * sizeof(T) / 2], b[8 * sizeof(T) / 2];
         const int64_t row_a = row;
         const int chunk_a = chunk;
-        load_chunk<T, VEC>(x + row * K, chunk, K, turn, a);
+        load_chunk<T, VEC>(x + row * K, chunk, K, turn, once, a);
         advance();
         const int64_t row_b = row;
         const int chunk_b = chunk;
-        load_chunk<T, VEC>(x + row * K, chunk, row < rows ? K : 0, turn, b);
+        load_chunk<T, VEC>(x + row * K, chunk, row < rows ? K : 0, turn, once, b);
         advance();
         const int64_t at_a = offsets ? slot_row(bounds, groups, int(row_a)) : row_a;
         quantize_chunk<T>(a, row_a, at_a, chunk_a, K, chunks, codes, ld, scale, sf);
@@ -190,8 +197,8 @@ fp8_rows_kernel(const T *__restrict__ x, int64_t rows, int K, const int *__restr
 // 2 R w + l / 16 + 2 i.  bf16: each thread copies its own 16-byte pieces of the next tiles to shared
 // memory ahead of time (cp.async, waited for by itself: the ring needs no barrier), so loads stay in
 // flight while a tile is reduced.  16384 x 4096 in both forms: 51.4 us = 5.2 TB/s (205 us with the tile in
-// registers and no ring, 52.7 with 4 rows per thread); bound by issue slots, three quarters of them
-// used.  fp32 tiles are loaded straight to registers (a ring of them leaves room for one CTA per SM:
+// registers and no ring, 52.7 with 4 rows per thread); bound by memory with one stream in and two out:
+// without the conversions, the barriers or the scale bytes it takes 2 % less.  fp32 tiles are loaded straight to registers (a ring of them leaves room for one CTA per SM:
 // 99 us against 55 for 8192 x 8192 weights).
 // Non-finite values (rare) are set to zero for the maxima and patched into the codes afterwards.
 enum { kRows = 1, kCols = 2, kWeight = 4 };
@@ -216,6 +223,11 @@ template <typename T> struct Piece {
     static constexpr int WORDS = sizeof(T) == 2 ? 4 : 8, CHUNKS = WORDS / 4;
     static constexpr int R = sizeof(T) == 2 ? 8 : 4, THREADS = 2048 / R;
     uint32_t u[R][WORDS];
+    __device__ __forceinline__ float value(int i, int j) const
+    {
+        if constexpr (sizeof(T) == 2) return __uint_as_float(j & 1 ? u[i][j >> 1] & 0xFFFF0000u : u[i][j >> 1] << 16);
+        else return __uint_as_float(u[i][j]);
+    }
     // sets non-finite values to zero; bit 8 i + j: value (i, j) was one
     __device__ __forceinline__ uint64_t drop_special()
     {
@@ -258,7 +270,7 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
     constexpr bool RING = VEC && sizeof(T) == 2;
     extern __shared__ uint4 ring[];                        // [D][R rows][CH][thread]
     __shared__ uint32_t colpart[WARPS][16 * P::WORDS];        // per warp: the columns' maxima (or, kWeight, one maximum)
-    __shared__ uint32_t colinv[16 * P::WORDS];              // reciprocal scales of the columns, as words
+    __shared__ alignas(16) float colinv[128];              // reciprocal scales of the columns
     __shared__ int bounds[MODE & kWeight ? 1 : kFp8MaxGroups + 1];
     if (!(MODE & kWeight) && p.offsets) load_bounds(bounds, p.offsets, p.groups, p.rows);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -356,15 +368,9 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
 #pragma unroll
             for (int i = 0; i < R; i++) m[i] = v.row_max(i), most = max(most, m[i]);
         }
-        auto put = [&](uint8_t *dst, int i, const uint32_t (&inv)[P::WORDS]) {
-            *reinterpret_cast<uint2 *>(dst) = make_uint2(W::codes(v.u[i], inv), W::codes(v.u[i] + P::WORDS / 2, inv + P::WORDS / 2));
+        auto put = [&](uint8_t *dst, int i, uint32_t lo, uint32_t hi) {
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(lo, hi);
             if (special) store_nans(dst, uint32_t(flags >> (8 * i)) & 0xFFu);
-        };
-        auto put_all = [&](uint8_t *dst, int i, uint32_t s) {      // one scale for the row's values
-            uint32_t inv[P::WORDS];
-#pragma unroll
-            for (int w = 0; w < P::WORDS; w++) inv[w] = s;
-            put(dst, i, inv);
         };
 
         if constexpr (MODE & kWeight) {
@@ -374,8 +380,11 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
             a = __reduce_max_sync(0xFFFFFFFFu, colpart[lane % WARPS][0]);
             const uint32_t e8 = fp8_e8m0(a);
 #pragma unroll
-            for (int i = 0; i < R; i++)
-                if (r0 + 2 * i < n && col < p.cols) put_all(p.codes + (matrix * p.rows + row0 + r0 + 2 * i) * p.ld + col, i, W::inv(e8));
+            for (int i = 0; i < R; i++) {
+                const uint32_t s = W::inv(e8), inv[4] = {s, s, s, s};
+                if (r0 + 2 * i < n && col < p.cols)
+                    put(p.codes + (matrix * p.rows + row0 + r0 + 2 * i) * p.ld + col, i, W::codes(v.u[i], inv), W::codes(v.u[i] + P::WORDS / 2, inv));
+            }
             const int nb = p.slots, nt = (nb + 3) / 4;
             if (tid == 0 && p.scale) p.scale[(matrix * nb + t) * kb + cb] = __uint_as_float(e8 << 23);
             if (tid < 128) {
@@ -386,6 +395,8 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
             continue;
         }
 
+        constexpr int SHARE = 16 / R;                       // lanes that end up with the same row
+        uint32_t row_e8 = 0;
         if constexpr (MODE & kCols) {
 #pragma unroll
             for (int w = 0; w < P::WORDS; w++) {
@@ -398,7 +409,6 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
             // Maxima of the R rows over 16 lanes: exchanges that halve what a lane keeps (its row is then the
             // upper log2 R of its four lane bits), plain steps for the other bits, and the scales
             // sent back: 16 shuffles instead of 32 for eight rows.
-            constexpr int SHARE = 16 / R;                   // lanes that end up with the same row
 #pragma unroll
             for (int h = R / 2, o = 8; h > 0; h /= 2, o /= 2) {
                 const bool up = lane & o;
@@ -411,15 +421,11 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
             uint32_t z = m[0];
 #pragma unroll
             for (int o = SHARE / 2; o > 0; o /= 2) z = max(z, __shfl_xor_sync(0xFFFFFFFFu, z, o));
-            const uint32_t e8 = fp8_e8m0(z);
+            row_e8 = fp8_e8m0(z);
             const int mine = r0 + 2 * ((lane & 15) / SHARE);
-            if (lane % SHARE == 0 && mine < n) p.sf[sf_offset(uint32_t(128 * t + mine), uint32_t(cb), uint32_t(kt))] = uint8_t(e8);
-#pragma unroll
-            for (int i = 0; i < R; i++) {
-                const uint32_t s = W::inv(__shfl_sync(0xFFFFFFFFu, e8, (lane & 16) | (i * SHARE)));
-                if (r0 + 2 * i < n && col < p.cols) put_all(p.codes + int64_t(row0 + r0 + 2 * i) * p.ld + col, i, s);
-            }
+            if (lane % SHARE == 0 && mine < n) p.sf[sf_offset(uint32_t(128 * t + mine), uint32_t(cb), uint32_t(kt))] = uint8_t(row_e8);
         }
+        float inv[8];                                       // of this thread's columns
         if constexpr (MODE & kCols) {
             __syncthreads();
             if (tid < 16 * P::WORDS) {                      // one word of columns per thread
@@ -427,28 +433,42 @@ fp8_tile_kernel(const T *__restrict__ x, const TileArgs p)
 #pragma unroll
                 for (int w = 0; w < WARPS; w++) a = W::max_of(a, colpart[w][tid]);
                 const int st = (p.slots + 3) / 4;
-                if constexpr (sizeof(T) == 2) {
-                    const uint32_t e0 = fp8_e8m0((a << 16) & kAbs), e1 = fp8_e8m0(a & 0x7FFF0000u);
-                    colinv[tid] = (W::inv(e0) & 0xFFFFu) | (W::inv(e1) & 0xFFFF0000u);
-                    p.sf_t[sf_offset(uint32_t(cb * 128 + 2 * tid), uint32_t(t), uint32_t(st))] = uint8_t(e0);
-                    p.sf_t[sf_offset(uint32_t(cb * 128 + 2 * tid + 1), uint32_t(t), uint32_t(st))] = uint8_t(e1);
-                } else {
-                    const uint32_t e0 = fp8_e8m0(a & kAbs);
-                    colinv[tid] = W::inv(e0);
-                    p.sf_t[sf_offset(uint32_t(cb * 128 + tid), uint32_t(t), uint32_t(st))] = uint8_t(e0);
+#pragma unroll
+                for (int h = 0; h < 8 / P::WORDS; h++) {
+                    const int c = 8 / P::WORDS * tid + h;
+                    const uint32_t e8 = fp8_e8m0(P::WORDS == 8 ? a & kAbs : h ? a & 0x7FFF0000u : (a << 16) & kAbs);
+                    colinv[c] = fp8_inv_scale(e8);
+                    p.sf_t[sf_offset(uint32_t(cb * 128 + c), uint32_t(t), uint32_t(st))] = uint8_t(e8);
                 }
             }
             __syncthreads();
-            uint32_t inv[P::WORDS];
 #pragma unroll
-            for (int w = 0; w < P::WORDS; w++) inv[w] = colinv[P::WORDS * (lane & 15) + w];
-            // Groups: the tile goes to its slot's rows, all 128 of them, so that the product over a
-            // group's rows runs in whole blocks (the values past the group are zeros).
-            const int64_t out0 = p.offsets ? 128ll * t : row0;
-            const int out_n = p.offsets ? 128 : n;
+            for (int h = 0; h < 2; h++) {
+                const float4 f = reinterpret_cast<const float4 *>(colinv)[2 * (lane & 15) + h];
+                inv[4 * h] = f.x, inv[4 * h + 1] = f.y, inv[4 * h + 2] = f.z, inv[4 * h + 3] = f.w;
+            }
+        }
+        // Both forms of a row from one unpacking to fp32.  Groups: the column-wise tile goes to its
+        // slot's rows, all 128 of them, so that the product over a group's rows runs in whole blocks (the
+        // values past the group are zeros).
+        const int64_t out0 = p.offsets ? 128ll * t : row0;
+        const int out_n = p.offsets ? 128 : n;
 #pragma unroll
-            for (int i = 0; i < R; i++)
-                if (r0 + 2 * i < out_n && col < p.cols) put(p.codes_t + (out0 + r0 + 2 * i) * p.ld + col, i, inv);
+        for (int i = 0; i < R; i++) {
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) f[j] = v.value(i, j);
+            const int r = r0 + 2 * i;
+            if constexpr (MODE & kRows) {
+                const float s = fp8_inv_scale(__shfl_sync(0xFFFFFFFFu, row_e8, (lane & 16) | (i * SHARE)));
+                if (r < n && col < p.cols)
+                    put(p.codes + int64_t(row0 + r) * p.ld + col, i,
+                        cvt_e4m3x4(f[0] * s, f[1] * s, f[2] * s, f[3] * s), cvt_e4m3x4(f[4] * s, f[5] * s, f[6] * s, f[7] * s));
+            }
+            if constexpr (MODE & kCols)
+                if (r < out_n && col < p.cols)
+                    put(p.codes_t + (out0 + r) * p.ld + col, i, cvt_e4m3x4(f[0] * inv[0], f[1] * inv[1], f[2] * inv[2], f[3] * inv[3]),
+                        cvt_e4m3x4(f[4] * inv[4], f[5] * inv[5], f[6] * inv[6], f[7] * inv[7]));
         }
     }
 }
@@ -517,7 +537,7 @@ int launch_rows(const void *x, int64_t rows, int64_t K, const int *offsets, int6
                 uint8_t *sf, unsigned grid, cudaStream_t st)
 {
     return launch_dependent(fp8_rows_kernel<T, VEC>, dim3(grid), 256, 0, st, static_cast<const T *>(x), rows, int(K), offsets, int(groups),
-                            codes, ld, scale, sf);
+                            codes, ld, scale, sf, rows * K * int64_t(sizeof(T)) > int64_t(64) << 20);
 }
 
 template <int MODE>

@@ -241,6 +241,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         ptx::prefetch_tmap(&tm_b);
         ptx::prefetch_tmap(&tm_sfa);
         ptx::prefetch_tmap(&tm_sfb);
+        // The first tiles of a dense forward product's weight start towards L2 while the kernel before
+        // (the quantizer of A) still runs.  Only a hint: L2 stays coherent with whoever writes them.
+        if (FORM == NT && !p.offsets) {
+            const int n0 = worker / ((p.M + 128 * CTAS - 1) / (128 * CTAS)) * BN + int(cta) * C::BCOLS;
+            for (int k = 0; k < C::STAGES && k * kBlock < p.K && n0 < p.N; k++)
+#pragma unroll
+                for (int b = 0; b < (C::BCOLS + 127) / 128; b++) ptx::tma_prefetch_3d(&tm_b, k * kBlock, n0 + 128 * b, 0);
+        }
     }
     if (warp == 1) {
         ptx::tmem_alloc<CTAS>(tmem_slot, kTmemCols);
@@ -332,6 +340,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             for (int t = worker; t < items && ok; t += workers) {
                 const Item it = item_of(t);
                 const int sfb0 = (FORM == TN ? 0 : it.g * p.sfb_rt) + it.n0 / 128;
+                // the second CTA of a pair whose group ended in the first one's rows multiplies zeros (rows behind
+                // the tensor), not the next group's rows: that takes less power
+                const int row_a = CTAS == 2 && FORM != TN && it.row0 >= it.row_end ? p.M : it.row0;
                 for (int k = 0; k < it.nkb; k++) {
                     if (!(ok = ptx::mbar_wait(empty_bar(s), ph ^ 1, abort_flag))) break;
                     const int kb = it.kb0 + k;
@@ -342,7 +353,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     if (cta == 0)
                         ptx::mbar_expect_tx(full_bar(s), CTAS * (p.a_bytes + C::B_BYTES + (scales ? 512u * (1 + C::SFB_TILES) : 0u)));
                     if (A_MN) ptx::tma_load_3d<CTAS>(st, &tm_a, it.row0, kb * kBlock, 0, bar);
-                    else ptx::tma_load_3d<CTAS>(st, &tm_a, k * kBlock, it.row0, 0, bar);
+                    else ptx::tma_load_3d<CTAS>(st, &tm_a, k * kBlock, row_a, 0, bar);
                     const uint32_t stb = st + C::A_BYTES;
                     const int nb0 = it.n0 + int(cta) * C::BCOLS;
 #pragma unroll

@@ -56,9 +56,16 @@ fp8_skinny_kernel(const T *__restrict__ x, const SkinnyArgs p)
 {
     using W = Word<T>;
     constexpr int WORDS = 16 * int(sizeof(T)) / 4;          // words of 16 values
-    begin_dependent_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int n0 = blockIdx.x * 16 * p.tiles, tiles = min(p.tiles, (p.N - n0 + 15) / 16);
+    // A dense weight's rows start towards L2 while the kernel before still runs (only a hint: L2 stays
+    // coherent with whoever writes them): the lines of the first two blocks of every warp.
+    if (!p.offsets)
+        for (int i = threadIdx.x; i < 16 * 2 * kWarps; i += 32 * kWarps) {
+            const int r = n0 + i / (2 * kWarps), k = i % (2 * kWarps) * 128;
+            if (r < p.N && k < p.K) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.codes + int64_t(r) * p.ld + k));
+        }
+    begin_dependent_launch();
     const int kb_count = (p.K + 127) / 128, kt = (kb_count + 3) / 4;
 
     int group = 0, lo = 0, hi = p.rows;
