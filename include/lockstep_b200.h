@@ -503,7 +503,8 @@ int ls_fp8_linear_backward(const void *gy, int dtype, int64_t rows, int64_t N, i
 int ls_fp8_linear_set_skinny(int on);
 
 /* For measurements and tests: 0 = choose by size (default); 1, 3, 4 = one CTA
- * per tile with 128, 64 (form 0 only, else 128), 256 columns; 2 = CTA pairs. */
+ * per tile with 128, 64 (form 0 only, else 128), 256 columns; 2 = CTA pairs;
+ * 5 = 128 columns with K split over four CTAs (dense products). */
 int ls_fp8_gemm_set_variant(int variant);
 
 #ifdef __cplusplus

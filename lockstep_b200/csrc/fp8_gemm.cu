@@ -31,6 +31,7 @@ namespace {
 constexpr int kThreads = 320;
 constexpr int kTmemCols = 512;
 constexpr int kBlock = 128;             // values of K per stage = per scale block
+constexpr int kMaxSplits = 4;           // CTAs of a cluster that share the K loop of a tile
 constexpr int kSegment = 32;            // blocks per accumulation chain of the LONG kernels
 enum Form { NT = 0, NN = 1, TN = 2 };
 
@@ -51,6 +52,8 @@ struct Fp8Cfg {
     static_assert(SFB_COL + 4 * SFB_TILES <= kTmemCols, "tensor memory overflow");
     static constexpr int STAGING = STAGES * STAGE_BYTES;   // of the epilogue warps; then barriers, the groups' tile prefix
     static constexpr int TAIL = STAGING + 8 * kStagingWords * 4;
+    // K split over a cluster of up to kMaxSplits CTAs: the others' sums of a tile lie over the stages of the first
+    static constexpr int PART_BYTES = 128 * BN * 4;
     static constexpr int LIST = TAIL + 256;
     static constexpr int SMEM = LIST + 4 * (kFp8MaxGroups + 4) + 1024;
     static_assert(STAGING % 1024 == 0, "swizzled tiles start on 1024-byte boundaries");
@@ -67,6 +70,7 @@ struct Fp8Params {
     int sfa_kt, sfb_kt;            // scale tiles along K per 128 rows of A / columns of B
     int sfb_rt;                    // NT, NN: 128-column scale tiles of one group's B
     int a_bytes;                   // what one load of an A tile delivers
+    int splits;                    // dense, single CTAs: CTAs per tile, each with its part of K (1: no split)
     int *err;
 };
 
@@ -183,11 +187,47 @@ __device__ __forceinline__ void store_rows(uint32_t stage, const CUtensorMap *ma
     }
 }
 
+// The parts of a tile's K loop meet in the cluster's shared memory, over the stages, which are free once
+// every CTA's MMAs are done.  The epilogue warps of one number share a piece of the tile; one of them,
+// a different CTA's for each number, adds the others' parts to its own in their order.  Called by the epilogue warps of all
+// CTAs, each with its part in `sum` (the other warps take part in the two cluster barriers); true for the
+// warp that has the result.  live: the piece has rows to store.
+template <int CH>
+__device__ __forceinline__ bool join(uint32_t smem_base, const uint8_t *gen_base, int warp, int lane, int part, int splits, bool live,
+                                     float (&sum)[CH][32])
+{
+    const int owner = warp % splits;
+    auto place = [&](int of) { return uint32_t(((of < owner ? of : of - 1) * 8 + warp) * CH * 4096 + lane * 4); };
+    __syncwarp();
+    cluster_sync();
+    if (part != owner && live) {
+        const uint32_t to = ptx::map_to_cta(smem_base + place(part), uint32_t(owner));
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int i = 0; i < 32; i++)
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + c * 4096 + i * 128), "f"(sum[c][i]) : "memory");
+    }
+    __syncwarp();
+    cluster_sync();
+    if (part != owner || !live) return false;
+    for (int of = 0; of < splits; of++) {
+        if (of == owner) continue;
+        const float *from = reinterpret_cast<const float *>(gen_base + place(of));
+#pragma unroll
+        for (int c = 0; c < CH; c++)
+#pragma unroll
+            for (int i = 0; i < 32; i++) sum[c][i] += from[c * 1024 + i * 32];
+    }
+    return true;
+}
+
 // One output tile of the CTA (pair): everything the three roles need.
 struct Item {
     int g;                         // group
     int row0, row_end;             // this CTA's first output row, and the end of the rows it may store
     int n0;                        // first output column
+    int k0;                        // first block of K of this CTA
     int kb0, nkb;                  // blocks of K: scale index of the first, count
     int slot;                      // this CTA's row tile in A's scale buffer
 };
@@ -198,7 +238,7 @@ struct Item {
 // kSegment blocks, each a chain of its own, that the epilogue adds in registers: 2.2e-7 after 16384
 // (torch's fp32 product: 3.6e-7) in 54 us for 4096 x 1024 outputs; segments half as long give 1.2e-7
 // in 57 us, one chain takes 51 us.
-template <int CTAS, int BN, int FORM, bool LONG>
+template <int CTAS, int BN, int FORM, bool LONG, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                 const __grid_constant__ CUtensorMap tm_sfa, const __grid_constant__ CUtensorMap tm_sfb,
@@ -206,6 +246,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 {
     using C = Fp8Cfg<CTAS, BN>;
     constexpr bool A_MN = FORM == TN, B_MN = FORM != NT;
+    static_assert(!SPLIT || (CTAS == 1 && (kMaxSplits - 1) * C::PART_BYTES <= C::STAGING), "partial sums overflow the stages");
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *gen_base = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
@@ -224,7 +265,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t cta = CTAS == 2 ? cluster_ctarank() : 0u;
-    const int worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
+    const int splits = SPLIT ? p.splits : 1, part = SPLIT ? int(cluster_ctarank()) : 0;
+    const int worker = blockIdx.x / (CTAS * splits), workers = gridDim.x / (CTAS * splits);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; s++) {
@@ -245,7 +287,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         // (the quantizer of A) still runs.  Only a hint: L2 stays coherent with whoever writes them.
         if (FORM == NT && !p.offsets) {
             const int n0 = worker / ((p.M + 128 * CTAS - 1) / (128 * CTAS)) * BN + int(cta) * C::BCOLS;
-            for (int k = 0; k < C::STAGES && k * kBlock < p.K && n0 < p.N; k++)
+            const int k0 = SPLIT ? part * (((p.K + kBlock - 1) / kBlock + splits - 1) / splits) : 0;
+            for (int k = k0; k < k0 + C::STAGES && k * kBlock < p.K && n0 < p.N; k++)
 #pragma unroll
                 for (int b = 0; b < (C::BCOLS + 127) / 128; b++) ptx::tma_prefetch_3d(&tm_b, k * kBlock, n0 + 128 * b, 0);
         }
@@ -328,6 +371,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
             it.kb0 = 0;
             it.nkb = (p.K + kBlock - 1) / kBlock;
         }
+        it.k0 = 0;
+        if (SPLIT) {                                        // dense: every part has blocks (the host sees to it)
+            const int per = (it.nkb + splits - 1) / splits;
+            it.k0 = part * per;
+            it.kb0 += it.k0;
+            it.nkb = min(it.nkb, it.k0 + per) - it.k0;
+        }
         return it;
     };
 
@@ -353,13 +403,13 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     if (cta == 0)
                         ptx::mbar_expect_tx(full_bar(s), CTAS * (p.a_bytes + C::B_BYTES + (scales ? 512u * (1 + C::SFB_TILES) : 0u)));
                     if (A_MN) ptx::tma_load_3d<CTAS>(st, &tm_a, it.row0, kb * kBlock, 0, bar);
-                    else ptx::tma_load_3d<CTAS>(st, &tm_a, k * kBlock, row_a, 0, bar);
+                    else ptx::tma_load_3d<CTAS>(st, &tm_a, (it.k0 + k) * kBlock, row_a, 0, bar);
                     const uint32_t stb = st + C::A_BYTES;
                     const int nb0 = it.n0 + int(cta) * C::BCOLS;
 #pragma unroll
                     for (int b = 0; b < (C::BCOLS + 127) / 128; b++) {
-                        if (!B_MN) ptx::tma_load_3d<CTAS>(stb + b * 128 * kBlock, &tm_b, k * kBlock, nb0 + 128 * b, it.g, bar);
-                        else if (FORM == NN) ptx::tma_load_3d<CTAS>(stb + b * 128 * kBlock, &tm_b, nb0 + 128 * b, k * kBlock, it.g, bar);
+                        if (!B_MN) ptx::tma_load_3d<CTAS>(stb + b * 128 * kBlock, &tm_b, (it.k0 + k) * kBlock, nb0 + 128 * b, it.g, bar);
+                        else if (FORM == NN) ptx::tma_load_3d<CTAS>(stb + b * 128 * kBlock, &tm_b, nb0 + 128 * b, (it.k0 + k) * kBlock, it.g, bar);
                         else ptx::tma_load_3d<CTAS>(stb + b * 128 * kBlock, &tm_b, nb0 + 128 * b, kb * kBlock, 0, bar);
                     }
                     if (scales) {
@@ -501,6 +551,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     }
                     if (C::OVL == 0) release();
                 }
+                if constexpr (SPLIT)
+                    if (!join<CH>(smem_base, gen_base, warp - 2, lane, part, splits, row < it.row_end, sum)) continue;
                 if (!ok) break;
 #pragma unroll
                 for (int c = 0; c < CH; c++) {
@@ -510,6 +562,30 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
                     emit(CH * half + c, r);
                 }
                 continue;
+            }
+            if constexpr (SPLIT) {
+                {                                           // one tile per CTA: nobody waits for this accumulator
+                    float sum[CH][32];
+                    ok = ptx::mbar_wait(acc_full_bar, 0, abort_flag);
+                    ptx::tc_fence_after();
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        uint32_t r[32];
+                        ptx::tmem_ld32(tmem_base + (uint32_t(32 * q) << 16) + 32 * (CH * half + c), r);
+                        ptx::tmem_ld_wait(r);
+#pragma unroll
+                        for (int i = 0; i < 32; i++) sum[c][i] = __uint_as_float(r[i]);
+                    }
+                    if (!join<CH>(smem_base, gen_base, warp - 2, lane, part, splits, row < it.row_end, sum) || !ok) continue;
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        uint32_t r[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i++) r[i] = __float_as_uint(sum[c][i]);
+                        emit(CH * half + c, r);
+                    }
+                    continue;
+                }
             }
             if (!(ok = ptx::mbar_wait(acc_full_bar + 8u * (lt & 1), (lt >> 1) & 1, abort_flag))) break;
             ptx::tc_fence_after();
@@ -585,6 +661,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
         }
     }
 
+    if (SPLIT && warp < 2) {                                // the other side of join()
+        __syncwarp();
+        cluster_sync();
+        cluster_sync();
+    }
+
     // ---------------------------------------------------------------- teardown
     if (*abort_flag) {
         for (int i = 0; i < 4096; i++) __nanosleep(256);    // copies and MMAs in flight land before memory is released
@@ -592,7 +674,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (CTAS == 2) cluster_sync();                          // neither CTA leaves while the other may still signal it
+    if (CTAS == 2 || SPLIT) cluster_sync();        // no CTA leaves while another may still signal or write to it
     if (warp == 1) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc<CTAS>(tmem_base, kTmemCols);
@@ -634,41 +716,71 @@ int make_map(CUtensorMap *m, const MapSpec &k)
     return LS_OK;
 }
 
-template <int CTAS, int BN, int FORM, bool LONG>
+template <int CTAS, int BN, int FORM, bool LONG, bool SPLIT>
 int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tsa, const CUtensorMap &tsb, const CUtensorMap &tc, const Fp8Params &p,
            int64_t most_tiles, cudaStream_t st)
 {
     using C = Fp8Cfg<CTAS, BN>;
     static int resident[64] = {};                           // CTAs (pairs) of this kernel that fit at once, per device
+    const unsigned cluster = unsigned(CTAS * p.splits);
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = CTAS, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
+    at[1].val.clusterDim.x = cluster, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = st;
     std::unique_lock<std::mutex> lk(state_mutex());
     if (!resident[dev]) {
-        LS_CUDA(cudaFuncSetAttribute(fp8_gemm_kernel<CTAS, BN, FORM, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        LS_CUDA(cudaFuncSetAttribute(fp8_gemm_kernel<CTAS, BN, FORM, LONG, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
         int n = sm_count();
         if (CTAS == 2) {
             cfg.gridDim = dim3(unsigned(sm_count() & ~1), 1, 1);
             cfg.attrs = at + 1, cfg.numAttrs = 1;
-            LS_CUDA(cudaOccupancyMaxActiveClusters(&n, fp8_gemm_kernel<CTAS, BN, FORM, LONG>, &cfg));
+            LS_CUDA(cudaOccupancyMaxActiveClusters(&n, fp8_gemm_kernel<CTAS, BN, FORM, LONG, SPLIT>, &cfg));
             if (n < 1) return fail(LS_ECUDA, "no CTA pair of the FP8 product fits on this device");
         }
         resident[dev] = n;
     }
-    const int64_t workers = std::max<int64_t>(1, std::min<int64_t>(most_tiles, resident[dev]));
+    // (a K split has one tile per cluster, and needs no two clusters at once)
+    const int64_t workers = p.splits > 1 ? most_tiles : std::max<int64_t>(1, std::min<int64_t>(most_tiles, resident[dev]));
     lk.unlock();
-    cfg.gridDim = dim3(unsigned(CTAS * workers), 1, 1);
-    cfg.attrs = at, cfg.numAttrs = CTAS == 2 ? 2 : 1;
-    LS_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<CTAS, BN, FORM, LONG>, ta, tb, tsa, tsb, tc, p));
+    cfg.gridDim = dim3(unsigned(cluster * workers), 1, 1);
+    cfg.attrs = at, cfg.numAttrs = cluster > 1 ? 2 : 1;
+    LS_CUDA(cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<CTAS, BN, FORM, LONG, SPLIT>, ta, tb, tsa, tsb, tc, p));
     return LS_OK;
+}
+
+// Clusters of `size` single CTAs that run at once on the current device (0: unknown).
+int cluster_room(int size)
+{
+    static int room[64][kMaxSplits + 1] = {};
+    int dev = 0;
+    if (current_device(&dev)) return 0;
+    std::lock_guard<std::mutex> lk(state_mutex());
+    if (!room[dev][size]) {
+        const auto kernel = fp8_gemm_kernel<1, 128, NT, false, true>;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = unsigned(size), at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(size) * 64, 1, 1);
+        cfg.blockDim = dim3(kThreads, 1, 1);
+        cfg.dynamicSmemBytes = Fp8Cfg<1, 128>::SMEM;
+        cfg.attrs = at, cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Fp8Cfg<1, 128>::SMEM) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        room[dev][size] = n;
+    }
+    return room[dev][size];
 }
 
 std::atomic<int> g_variant{0};          // 0 = choose by size; else see ls_fp8_gemm_set_variant
@@ -720,26 +832,41 @@ int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t 
     // 768, 128 x 128 512, 128 x 64 (K-major B only) 384.  Among equals the smaller tile, whose epilogue is
     // shorter (2048 x 1024 over 4999 rows: 12.6 us against 17.0 of the pair's).  A ragged group ends in
     // half a tile on average.  With few rows per group the second CTA of a pair idles: no pairs there.
-    const int variant = g_variant.load(std::memory_order_relaxed);
+    const int variant = g_variant.load(std::memory_order_relaxed), sms = sm_count();
+    p.splits = 1;
     const bool by_rows = form != TN && offsets;
     auto tiles = [&](int64_t rows, int64_t cols, int64_t part) {       // part / 2 of a tile more per group
         const int64_t m = by_rows ? M / rows + (part * groups + 1) / 2 : (M + rows - 1) / rows;
         return m * ((N + cols - 1) / cols) * (form == TN ? groups : 1);
     };
+    // K split: the CTAs of a cluster take parts of a dense tile's K loop, while all clusters run at once (74 of
+    // two, 45 of three, 33 of four CTAs: the SMs of a cluster are neighbours); their sums meet in shared
+    // memory, which takes about 3500 + 400 cycles per part with 64 columns and 3000 + 1500 with 128.  A
+    // split is taken where it promises a sixth or more.  16 rows, 16384 -> 2048: 27.6 -> 12.8 us; weight
+    // gradient of 512 x 512 over 16384 rows: 30.5 -> 14.9; 16 rows, 4096 -> 4096: 9.4 -> 8.9.
+    const int64_t nkb = (K + kBlock - 1) / kBlock;
     bool pair = variant == 2;
     int bn = variant == 4 || variant == 2 ? 256 : variant == 3 && form == NT ? 64 : 128;
+    if (variant == 5) p.splits = int(std::min<int64_t>(kMaxSplits, nkb));
     if (variant == 0) {
         int64_t best = -1;
-        auto consider = [&](bool p2, int cols, int64_t cycles) {
-            const int64_t workers = p2 ? sm_count() / 2 : sm_count();
-            const int64_t cost = (tiles(p2 ? 256 : 128, cols, 1) + workers - 1) / workers * cycles;
-            if (best < 0 || cost < best) best = cost, pair = p2, bn = cols;
+        auto consider = [&](bool p2, int cols, int64_t cycles, int splits) {
+            const int64_t workers = p2 ? sms / 2 : sms, n = tiles(p2 ? 256 : 128, cols, 1) * splits;
+            if (splits > 1 && (offsets || n > int64_t(splits) * cluster_room(splits) || nkb < splits)) return;
+            int64_t cost = cycles * ((nkb + splits - 1) / splits);
+            if (splits == 1) cost *= (n + workers - 1) / workers;
+            else cost = (cost + (cols == 64 ? 3500 + 400 * splits : 3000 + 1500 * splits)) * 7 / 6;
+            if (best < 0 || cost < best) best = cost, pair = p2, bn = cols, p.splits = splits;
         };
-        if (form == NT) consider(false, 64, 384);
-        consider(false, 128, 512);
-        consider(false, 256, 768);
-        if (M > (by_rows ? 128 * groups : 128)) consider(true, 256, 512);
+        for (int splits = 1; splits <= kMaxSplits; splits++) {
+            if (form == NT) consider(false, 64, 384, splits);
+            consider(false, 128, 512, splits);
+        }
+        consider(false, 256, 768, 1);
+        if (M > (by_rows ? 128 * groups : 128)) consider(true, 256, 512, 1);
     }
+    if (offsets || pair || bn == 256) p.splits = 1;
+    if (p.splits > 1) p.splits = int((nkb + (nkb + p.splits - 1) / p.splits - 1) / ((nkb + p.splits - 1) / p.splits));    // no empty part
     const int64_t items = tiles(pair ? 256 : 128, bn, 2);
     if (items > 0x7FFFFFFFll) return fail(LS_EINVAL, "too many output tiles");
     const int64_t a_tiles = fp8_sf_tiles(form == TN ? M : slots * 128, kblocks);
@@ -767,15 +894,21 @@ int fp8_gemm(int form, const uint8_t *a, int64_t lda, const uint8_t *b, int64_t 
     if (N * es % 16 == 0)
         if (int rc = make_map(&tc, {c, N, M, form == TN ? groups : 1, N * es, int(128 / es), 16, p.out_bf16 ? kMapBf16 : kMapF32})) return rc;
     const bool many = out_dtype == LS_F32 && kblocks > kSegment;
-#define LS_FP8_LAUNCH(C, B, F) \
-    return many ? launch<C, B, F, true>(ta, tb, tsa, tsb, tc, p, items, st) : launch<C, B, F, false>(ta, tb, tsa, tsb, tc, p, items, st)
-#define LS_FP8_FORM(F)                          \
-    if (form == F) {                            \
-        if (pair) LS_FP8_LAUNCH(2, 256, F);     \
-        if (bn == 256) LS_FP8_LAUNCH(1, 256, F); \
-        LS_FP8_LAUNCH(1, 128, F);               \
+    const bool split = p.splits > 1;
+#define LS_FP8_LAUNCH(C, B, F, S)                                                    \
+    return many ? launch<C, B, F, true, S>(ta, tb, tsa, tsb, tc, p, items, st)       \
+                : launch<C, B, F, false, S>(ta, tb, tsa, tsb, tc, p, items, st)
+#define LS_FP8_FORM(F)                                  \
+    if (form == F) {                                    \
+        if (pair) LS_FP8_LAUNCH(2, 256, F, false);      \
+        if (bn == 256) LS_FP8_LAUNCH(1, 256, F, false); \
+        if (split) LS_FP8_LAUNCH(1, 128, F, true);      \
+        LS_FP8_LAUNCH(1, 128, F, false);                \
     }
-    if (form == NT && bn == 64) LS_FP8_LAUNCH(1, 64, NT);
+    if (form == NT && bn == 64) {
+        if (split) LS_FP8_LAUNCH(1, 64, NT, true);
+        LS_FP8_LAUNCH(1, 64, NT, false);
+    }
     LS_FP8_FORM(NT)
     LS_FP8_FORM(NN)
     LS_FP8_FORM(TN)
@@ -805,7 +938,7 @@ extern "C" int ls_fp8_gemm_grouped(int form, const uint8_t *a, int64_t lda, cons
 
 extern "C" int ls_fp8_gemm_set_variant(int variant)
 {
-    if (variant < 0 || variant > 4) return fail(LS_EINVAL, "variant must be 0..4");
+    if (variant < 0 || variant > 5) return fail(LS_EINVAL, "variant must be 0..5");
     g_variant.store(variant, std::memory_order_relaxed);
     return LS_OK;
 }

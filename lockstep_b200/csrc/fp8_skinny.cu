@@ -254,8 +254,8 @@ fp8_skinny_kernel(const T *__restrict__ x, const SkinnyArgs p)
     }
 }
 
-constexpr int kRingBytes = kAhead * 4 * 32 * kWarps * 16, kMaxX = 48 * 1024;
-constexpr int kMaxSmem = 160 * 1024;
+constexpr int kRingBytes = kAhead * 4 * 32 * kWarps * 16, kMaxX = 72 * 1024;
+constexpr int kMaxSmem = 200 * 1024;
 
 size_t x_bytes(int64_t rows, int64_t K)
 {
@@ -300,10 +300,11 @@ bool fp8_skinny_fits(int64_t rows, int64_t N, int64_t K, int64_t groups)
 int fp8_skinny_linear(const void *x, int dtype, int64_t rows, int64_t K, const uint8_t *codes, int64_t ld, const uint8_t *sf, int64_t N,
                       void *y, int out_dtype, const int *offsets, int64_t groups, int zero_tail, cudaStream_t st)
 {
-    // tiles per CTA: what leaves three CTAs per SM, within the shared memory of two
+    // tiles per CTA: what leaves as many CTAs per SM as x leaves room for, three at most
     const int64_t units = (N + 15) / 16 * (offsets ? std::min(groups, rows) : 1);
-    int64_t tiles = std::min<int64_t>({units / (3 * sm_count()) + 1, kMaxTiles, (N + 15) / 16});
-    while (tiles > 1 && kRingBytes + x_bytes(rows, K) + tiles * tile_bytes(K) > 110 * 1024) tiles--;
+    const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(3, 220 * 1024 / (kRingBytes + x_bytes(rows, K) + tile_bytes(K))));
+    int64_t tiles = std::min<int64_t>({units / (per_sm * sm_count()) + 1, kMaxTiles, (N + 15) / 16});
+    while (tiles > 1 && (kRingBytes + x_bytes(rows, K) + tiles * tile_bytes(K)) * per_sm > 224 * 1024) tiles--;
     const SkinnyArgs p{int(rows), int(K), int(N), codes, ld, sf, y, out_dtype == LS_BF16, offsets, int(groups), zero_tail, int(tiles)};
     const bool vec = aligned16(x) && K * (dtype == LS_BF16 ? 2 : 4) % 16 == 0;
     if (dtype == LS_BF16) return vec ? launch<__nv_bfloat16, true>(x, p, st) : launch<__nv_bfloat16, false>(x, p, st);

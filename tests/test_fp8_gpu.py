@@ -125,7 +125,7 @@ def _variant(v):
     check(lib().ls_fp8_gemm_set_variant(v))
 
 
-@pytest.fixture(params=[0, 1, 2, 3, 4])
+@pytest.fixture(params=[0, 1, 2, 3, 4, 5])
 def variant(request):
     _variant(request.param)
     yield request.param
@@ -447,7 +447,7 @@ def test_abi_refusals():
     assert L.ls_fp8_linear_forward(p, 0, p, 0, 4, 4, 128, None, 1, 3, p, None, p, stream()) == EINVAL       # nowhere to keep
     assert L.ls_fp8_linear_forward(p, 0, p, 0, 4, 4, 128, None, 1, 4, p, p, p, stream()) == EINVAL
     assert L.ls_fp8_gemm_grouped(0, p, 128, p, 128, p, p, p, 0, 4, 4, 0, ptr(off), 1, 0, stream()) == EINVAL
-    assert L.ls_fp8_gemm_set_variant(5) == EINVAL
+    assert L.ls_fp8_gemm_set_variant(6) == EINVAL
     torch.cuda.synchronize()
 
 
