@@ -40,43 +40,43 @@ def _buffer_bytes(what, rows, N, K, groups, grads):
     return int(lib().ls_fp8_linear_bytes(what, rows, N, K, groups, grads))
 
 
-def _buffer(what, rows, N, K, groups, grads, device):
-    n = _buffer_bytes(what, rows, N, K, groups, grads)
-    if n == 0 and what == _SERVE:                              # a few rows need no buffer
-        return None
-    return torch.empty((max(n, 16),), dtype=torch.uint8, device=device)
+@functools.lru_cache(maxsize=4096)
+def _training_bytes(rows, N, K, groups, grads):
+    """Buffers of a forward pass, kept for the backward pass, of a backward pass."""
+    return tuple(max(16, _buffer_bytes(what, rows, N, K, groups, grads)) for what in (_FORWARD, _SAVED, _BACKWARD))
 
 
 class _FP8Matmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
         with on_device_of(x, w, offsets):
-            off, G = fp8._groups(offsets)
+            off, G = (None, 0) if offsets is None else fp8._groups(offsets)
             if off is not None and w.shape[0] != G:
                 raise AssertionError(f"{w.shape[0]} experts for offsets of {G} groups")
             xi, wi = fp8._aligned(x), fp8._input(w, w.dim())
-            (rows, K), N, dev = xi.shape, w.shape[-2], x.device
-            grads = (_GRAD_X if ctx.needs_input_grad[0] else 0) | (_GRAD_W if ctx.needs_input_grad[1] else 0)
-            y = torch.empty((rows, N), dtype=x.dtype, device=dev)
-            work = _buffer(_FORWARD, rows, N, K, G, grads, dev)
-            saved = _buffer(_SAVED, rows, N, K, G, grads, dev) if grads else None
+            (rows, K), N = xi.shape, w.shape[-2]
+            need = ctx.needs_input_grad
+            grads = (_GRAD_X if need[0] else 0) | (_GRAD_W if need[1] else 0)
+            work_bytes, saved_bytes, back_bytes = _training_bytes(rows, N, K, G, grads)
+            y = xi.new_empty((rows, N))
+            work = xi.new_empty((work_bytes,), dtype=torch.uint8)
+            saved = xi.new_empty((saved_bytes,), dtype=torch.uint8) if grads else None
             check(lib().ls_fp8_linear_forward(xi.data_ptr(), fp8._DTYPE[xi.dtype], wi.data_ptr(), fp8._DTYPE[wi.dtype], rows, N, K,
-                                              fp8._ptr(off), G or 1, grads, y.data_ptr(), fp8._ptr(saved), work.data_ptr(), fp8._stream(x)))
+                                              fp8._ptr(off), G or 1, grads, y.data_ptr(), fp8._ptr(saved), work.data_ptr(), fp8._stream(xi)))
             ctx.save_for_backward(saved, off)
-            ctx.what = (rows, N, K, G, grads, x.dtype, w.dtype, w.shape)
+            ctx.what = (rows, N, K, G, grads, x.dtype, w.dtype, w.shape, back_bytes)
             return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
         saved, off = ctx.saved_tensors
-        rows, N, K, G, grads, x_dtype, w_dtype, w_shape = ctx.what
+        rows, N, K, G, grads, x_dtype, w_dtype, w_shape, back_bytes = ctx.what
         with on_device_of(gy, saved, off):
             gy = fp8._input(gy)
-            dev = gy.device
-            gx = torch.empty((rows, K), dtype=x_dtype, device=dev) if grads & _GRAD_X else None
-            gw = torch.empty(w_shape, dtype=w_dtype if w_dtype in fp8._DTYPE else torch.float32, device=dev) if grads & _GRAD_W else None
-            work = _buffer(_BACKWARD, rows, N, K, G, grads, dev)
+            gx = gy.new_empty((rows, K), dtype=x_dtype) if grads & _GRAD_X else None
+            gw = gy.new_empty(w_shape, dtype=w_dtype if w_dtype in fp8._DTYPE else torch.float32) if grads & _GRAD_W else None
+            work = gy.new_empty((back_bytes,), dtype=torch.uint8)
             check(lib().ls_fp8_linear_backward(gy.data_ptr(), fp8._DTYPE[gy.dtype], rows, N, K, fp8._ptr(off), G or 1, grads,
                                                saved.data_ptr(), fp8._ptr(gx), fp8._DTYPE[x_dtype], fp8._ptr(gw),
                                                _lib.LS_F32 if gw is None else fp8._DTYPE[gw.dtype], work.data_ptr(), fp8._stream(gy)))
@@ -119,7 +119,8 @@ def _serve(x, codes, sf, offsets, out_dtype, out):
             out_dtype = x.dtype
         code = fp8._out_code(out_dtype)
         y = x.new_empty((rows, N), dtype=out_dtype) if out is None else fp8._given(out, (rows, N), out_dtype)
-        work = _buffer(_SERVE, rows, N, K, G, 0, x.device)
+        size = _buffer_bytes(_SERVE, rows, N, K, G, 0)
+        work = x.new_empty((size,), dtype=torch.uint8) if size else None       # (a few rows need no buffer)
         check(lib().ls_fp8_linear(x.data_ptr(), fp8._DTYPE[x.dtype], rows, K, codes.data_ptr(), ld, sf.data_ptr(), N, y.data_ptr(), code,
                                   fp8._ptr(off), G or 1, 1 if out is None else 0, fp8._ptr(work), fp8._stream(x)))
         return y
