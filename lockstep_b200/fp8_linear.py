@@ -48,7 +48,8 @@ def _training_bytes(rows, N, K, groups, grads):
 
 class _FP8Matmul(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, offsets):
+    def forward(ctx, x, w, offsets, recording):
+        # recording: the caller's grad mode; without it nothing is prepared for a backward pass
         with on_device_of(x, w, offsets):
             off, G = (None, 0) if offsets is None else fp8._groups(offsets)
             if off is not None and w.shape[0] != G:
@@ -56,7 +57,7 @@ class _FP8Matmul(torch.autograd.Function):
             xi, wi = fp8._aligned(x), fp8._input(w, w.dim())
             (rows, K), N = xi.shape, w.shape[-2]
             need = ctx.needs_input_grad
-            grads = (_GRAD_X if need[0] else 0) | (_GRAD_W if need[1] else 0)
+            grads = (_GRAD_X if need[0] else 0) | (_GRAD_W if need[1] else 0) if recording else 0
             work_bytes, saved_bytes, back_bytes = _training_bytes(rows, N, K, G, grads)
             y = xi.new_empty((rows, N))
             work = xi.new_empty((work_bytes,), dtype=torch.uint8)
@@ -80,15 +81,15 @@ class _FP8Matmul(torch.autograd.Function):
             check(lib().ls_fp8_linear_backward(gy.data_ptr(), fp8._DTYPE[gy.dtype], rows, N, K, fp8._ptr(off), G or 1, grads,
                                                saved.data_ptr(), fp8._ptr(gx), fp8._DTYPE[x_dtype], fp8._ptr(gw),
                                                _lib.LS_F32 if gw is None else fp8._DTYPE[gw.dtype], work.data_ptr(), fp8._stream(gy)))
-            return gx, (gw if gw is None or gw.dtype == w_dtype else gw.to(w_dtype)), None
+            return gx, (gw if gw is None or gw.dtype == w_dtype else gw.to(w_dtype)), None, None
 
 
 def linear(x, weight):
     """x [..., in] (bf16 or fp32), weight [out, in] -> [..., out] in x's dtype, with FP8 gradients."""
     _check(x, weight, 2)
     if x.dim() == 2:
-        return _FP8Matmul.apply(x, weight, None)
-    return _FP8Matmul.apply(x.reshape(-1, x.shape[-1]), weight, None).view(*x.shape[:-1], weight.shape[0])
+        return _FP8Matmul.apply(x, weight, None, torch.is_grad_enabled())
+    return _FP8Matmul.apply(x.reshape(-1, x.shape[-1]), weight, None, torch.is_grad_enabled()).view(*x.shape[:-1], weight.shape[0])
 
 
 def grouped_linear(x, weight, offsets):
@@ -99,7 +100,7 @@ def grouped_linear(x, weight, offsets):
         raise AssertionError(f"rows sorted by expert are two-dimensional, got shape {tuple(x.shape)}")
     if offsets is None:
         raise AssertionError("offsets are needed")
-    return _FP8Matmul.apply(x, weight, offsets)
+    return _FP8Matmul.apply(x, weight, offsets, torch.is_grad_enabled())
 
 
 # One token's linear is a few microseconds on the device, so these two keep to what the call needs;

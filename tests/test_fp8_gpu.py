@@ -624,6 +624,31 @@ def test_training_step_captured():
     assert torch.equal(got[0], ref_grads[0]) and torch.equal(got[1], ref_grads[1])
 
 
+def test_nothing_is_kept_without_gradients():
+    from lockstep_b200 import fp8_linear
+    rows, K, N = 4096, 2048, 256
+    x, w = _data(rows, K, seed=35).requires_grad_(), _data(N, K, seed=36).requires_grad_()
+    off = _offsets([1000, rows - 1000])
+    wg = torch.stack([w.detach(), -w.detach()]).requires_grad_()
+    for f, experts in ((lambda: fp8_linear.linear(x, w), 1), (lambda: fp8_linear.grouped_linear(x, wg, off), 2)):
+        want = f()
+        kept = want.detach().clone()
+        del want
+        for mode in (torch.no_grad, torch.inference_mode):
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            with mode():
+                y = f()
+            torch.cuda.synchronize()
+            peak = torch.cuda.max_memory_allocated() - before
+            # one byte per value, the scales (a 32nd of that at most) and the output; half of x's codes again is too much
+            values = (rows + experts * 128) * K + experts * N * K
+            assert peak < values * 33 // 32 + y.numel() * y.element_size() + rows * K // 2, (peak, values)
+            assert torch.equal(y, kept)
+            del y
+
+
 def test_first_call_of_a_process_may_be_captured():
     import subprocess
     import sys
